@@ -1,0 +1,363 @@
+// The 8-bit entry points of libsgemm_runner.so (include/sgemm_runner.h, "8-bit operands"): argument checks, the choice
+// of kernel and cut, tensor maps and launches.  They work on handles of cubins generated for INT8 operands.
+//
+// Every call is one launch.  None of them uses the handle's workspace or keeps anything between calls: tensor maps are made
+// anew from the arguments and travel as kernel arguments, parts of a cut sum meet in shared memory.  So calls on several
+// streams, and captured graphs replayed side by side, need no ordering among themselves beyond that of their data.
+#include "sgemm_internal.hpp"
+#include "sgemm_i8_params.hpp"
+
+#include <algorithm>
+#include <cstdio>
+#include <cstring>
+
+#define SGEMM_API extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+using namespace sgemm_internal;
+
+constexpr uint32_t kSmsPerPair = 2;
+
+// index of a kernel in the handle's table; the row kernels follow as [operation][type][form]
+enum : int {
+    kFew16 = 0, kFew32, kFew64, kFew128, kWgrad, kWgradSimt, kLinear, kLinearSimt,
+    kQuantize,                                   // + 4 * type + form (vectors per thread 1, 2, 4; single elements)
+    kNorm = kQuantize + 12,
+    kRestore = kNorm + 12,                       // + 2 * type + (0 vectors, 1 single elements)
+    kCount = kRestore + 6
+};
+static_assert(kCount <= kI8Functions, "the handle's table holds every kernel");
+
+const char *const kNames[kCount] = {
+    "i8_linear_few_16", "i8_linear_few_32", "i8_linear_few_64", "i8_linear_few_128", "i8_wgrad", "i8_wgrad_simt",
+    "generated_gemm", "generated_gemm_simt",
+    "i8_quantize_fp32_v1", "i8_quantize_fp32_v2", "i8_quantize_fp32_v4", "i8_quantize_fp32_s4",
+    "i8_quantize_fp16_v1", "i8_quantize_fp16_v2", "i8_quantize_fp16_v4", "i8_quantize_fp16_s4",
+    "i8_quantize_bf16_v1", "i8_quantize_bf16_v2", "i8_quantize_bf16_v4", "i8_quantize_bf16_s4",
+    "i8_rmsnorm_fp32_v1", "i8_rmsnorm_fp32_v2", "i8_rmsnorm_fp32_v4", "i8_rmsnorm_fp32_s4",
+    "i8_rmsnorm_fp16_v1", "i8_rmsnorm_fp16_v2", "i8_rmsnorm_fp16_v4", "i8_rmsnorm_fp16_s4",
+    "i8_rmsnorm_bf16_v1", "i8_rmsnorm_bf16_v2", "i8_rmsnorm_bf16_v4", "i8_rmsnorm_bf16_s4",
+    "i8_restore_fp32_v", "i8_restore_fp32_s", "i8_restore_fp16_v", "i8_restore_fp16_s", "i8_restore_bf16_v", "i8_restore_bf16_s",
+};
+
+struct FewKernel {
+    int index;
+    uint32_t tile_n, smem;
+};
+const FewKernel kFew[] = {
+    {kFew16, 16, I8_FEW_SMEM(16, I8_FEW_STAGES_16)},
+    {kFew32, 32, I8_FEW_SMEM(32, I8_FEW_STAGES_32)},
+    {kFew64, 64, I8_FEW_SMEM(64, I8_FEW_STAGES_64)},
+    {kFew128, 128, I8_FEW_SMEM(128, I8_FEW_STAGES_128)},
+};
+
+// mirrors of the kernels' argument structures
+struct LinearArgs {
+    const void *w, *sw, *x, *sx, *bias;
+    void *y;
+    uint32_t *status;
+    uint32_t m, n, k, ldw, ldx, ldy, y_type, tiles_m, tiles_n;
+};
+struct WgradArgs {
+    const void *q, *scale, *g, *c;
+    void *d;
+    uint32_t *status;
+    uint32_t m, n, tokens, ldq, ldg, ldc, ldd, g_type, d_type;
+    float alpha, beta;
+    uint32_t tiles_m, tiles_n;
+};
+struct RowArgs {
+    const void *x, *r, *g;
+    void *sum, *q, *scale;
+    uint32_t k, rows, ldx, ldr, lds, ldq, tpr, pow2;
+    float eps;
+};
+
+int refuse(sgemm_handle *h, int code, const char *op, const char *what) {
+    char text[256];
+    std::snprintf(text, sizeof text, "%s: %s", op, what);
+    return set_error(h, code, text);
+}
+uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }   // (a + b - 1 stays below 2^32: callers bound a)
+bool aligned(const void *p, size_t bytes) { return ((uintptr_t)p % bytes) == 0; }
+uint32_t type_bytes(int type) { return type == (int)SGEMM_I8_FP32 ? 4u : 2u; }
+bool known_type(int type) { return type >= 0 && type <= 2; }
+
+// what every entry point checks first
+int begin(sgemm_handle *h, const char *op, I8View *v) {
+    if (!h) return SGEMM_ERR_INVALID_ARGUMENT;
+    if (!i8_view(h, v)) return refuse(h, SGEMM_ERR_UNSUPPORTED, op, "the loaded cubin is not one for INT8 operands");
+    return SGEMM_OK;
+}
+
+constexpr uint32_t kLargest = 0xFFFFFF00u;   // sizes above this would wrap when rounded up to a tile
+
+// ---------------------------------------------------------------------------------------------- linear
+struct LinearPlan {
+    int index = kLinear;
+    const FewKernel *few = nullptr;
+    uint32_t parts = 1;
+};
+
+// Parts of K for the few-token kernel: the cut with the least work on the longest-running SM.  A CTA costs its stages plus a
+// fixed share (set-up, first loads, reduction: about four stages); `slots` of them run at a time.
+uint32_t cut_k(uint32_t tiles, uint32_t stages, uint32_t slots, uint64_t *cost) {
+    uint32_t best = 1;
+    uint64_t best_cost = ~0ull;
+    for (uint32_t parts = 1; parts <= 8 && parts <= std::max(1u, stages / 2); parts *= 2) {
+        const uint64_t waves = ((uint64_t)tiles * parts + slots - 1) / slots;
+        const uint64_t c = waves * (ceil_div(stages, parts) + 4);
+        if (c < best_cost) { best_cost = c; best = parts; }
+    }
+    if (cost) *cost = best_cost;
+    return best;
+}
+
+int plan_linear(sgemm_handle *h, const I8View &v, const void *w, const void *x, uint32_t m, uint32_t n, uint32_t k,
+                uint32_t ldw, uint32_t ldx, LinearPlan *p) {
+    const bool tma = aligned(w, 16) && aligned(x, 16) && ldw % 16 == 0 && ldx % 16 == 0;
+    if (v.force_variant == 1 || v.force_variant == 3) {
+        if (!tma || k == 0)
+            return refuse(h, SGEMM_ERR_UNSUPPORTED, "sgemm_i8_linear",
+                          "a tensor kernel is forced but the operands need 16-byte aligned bases, leading dimensions that are multiples of 16 and K > 0");
+    }
+    if (v.force_variant == 2 || !tma || k == 0) {
+        p->index = kLinearSimt;
+        return SGEMM_OK;
+    }
+    const uint32_t sms = (uint32_t)std::max(v.sm_count, 2), stages = ceil_div(k, I8_BK);
+    const uint32_t pairs_m = ceil_div(m, 256), pairs_n = ceil_div(n, v.tile_n);
+    // the few-token kernel whose tile holds all tokens, else the widest
+    const FewKernel *few = &kFew[3];
+    for (const FewKernel &f : kFew)
+        if (n <= f.tile_n) { few = &f; break; }
+    const uint64_t few_tiles = (uint64_t)ceil_div(m, I8_BM) * ceil_div(n, few->tile_n);
+    bool use_few = v.force_variant == 3;
+    uint32_t parts = 1;
+    if (v.force_variant != 1 && few_tiles * 8 < 0x7FFFFFFFull) {
+        uint64_t few_cost = 0;
+        parts = cut_k((uint32_t)few_tiles, stages, sms * (few->tile_n <= 64 ? 2 : 1), &few_cost);
+        // a pair's stage is 256 x 256 x 128 in 512 tensor cycles, a 128 x 128 one about 320 (bound by shared memory)
+        const uint64_t pair_waves = ((uint64_t)pairs_m * pairs_n + sms / kSmsPerPair - 1) / (sms / kSmsPerPair);
+        if (!use_few) use_few = n <= 128 || few_cost * 320 < pair_waves * (stages + 6) * 512;
+        if (v.split_k > 0) parts = v.split_k >= 8 ? 8u : v.split_k >= 4 ? 4u : v.split_k >= 2 ? 2u : 1u;
+    }
+    if (use_few) {
+        p->index = few->index;
+        p->few = few;
+        p->parts = parts;
+    }
+    return SGEMM_OK;
+}
+
+// ------------------------------------------------------------------------------------------ row kernels
+// Threads per row and vectors per thread: the fewest threads that hold the row in four vectors each, then, while all rows
+// together would leave SMs without a block, twice as many threads with half the vectors.
+void plan_rows(const I8View &v, uint32_t k, uint32_t rows, uint32_t per_vector, bool vec, uint32_t *tpr, int *form) {
+    const uint32_t vectors = std::max(1u, (k + per_vector - 1) / per_vector);
+    uint32_t nv = 4, threads = 32;
+    while (threads < I8_ROW_MAX_THREADS && (uint64_t)threads * nv < vectors) threads *= 2;
+    if (vec)
+        while (nv > 1 && threads < I8_ROW_MAX_THREADS && (uint64_t)threads * nv >= vectors &&
+               (uint64_t)rows * threads < (uint64_t)v.sm_count * 2048) {
+            threads *= 2;
+            nv /= 2;
+        }
+    while (nv > 1 && vec && (uint64_t)threads * (nv / 2) >= vectors) nv /= 2;
+    *tpr = threads;
+    *form = !vec ? 3 : nv == 4 ? 2 : nv == 2 ? 1 : 0;
+}
+
+int launch_rows(sgemm_handle *h, const I8View &v, int base, int type, bool vec, RowArgs &a, void *stream) {
+    int form = 0;
+    plan_rows(v, a.k, a.rows, 16 / type_bytes(type), vec, &a.tpr, &form);
+    const uint32_t threads = std::max<uint32_t>(I8_ROW_THREADS, a.tpr), per_block = threads / a.tpr;
+    void *params[] = {&a};
+    return i8_launch(h, v.functions[base + 4 * type + form], ceil_div(a.rows, per_block), threads, 0, 0, stream, params);
+}
+
+}  // namespace
+
+namespace sgemm_internal {
+
+int i8_function_count() { return kCount; }
+const char *i8_function_name(int index) { return kNames[index]; }
+uint32_t i8_function_smem(int index, uint32_t main_smem) {
+    for (const FewKernel &f : kFew)
+        if (f.index == index) return f.smem;
+    return index == kWgrad ? (uint32_t)I8W_SMEM : index == kLinear ? main_smem : 0u;
+}
+int i8_function_registers(int index) { return index == kWgrad ? I8W_LAUNCH_REGS : 0; }
+
+}  // namespace sgemm_internal
+
+SGEMM_API int sgemm_i8_linear(sgemm_handle *h, const int8_t *dW, const float *dWscale, const int8_t *dX, const float *dXscale,
+                              const float *dBias, void *dY, int y_type, uint32_t m, uint32_t n, uint32_t k, uint32_t ldw,
+                              uint32_t ldx, uint32_t ldy, void *stream) {
+    const char *op = "sgemm_i8_linear";
+    I8View v;
+    int rc = begin(h, op, &v);
+    if (rc) return rc;
+    if (!known_type(y_type)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "Y's type is FP32 (0), FP16 (1) or BF16 (2)");
+    if (k > I8_MAX_K) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "K above 131071: the 32-bit integer sum could overflow");
+    if (ldw < std::max(k, 1u) || ldx < std::max(k, 1u) || ldy < std::max(m, 1u))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a leading dimension is smaller than the rows it must hold");
+    if (m == 0 || n == 0) return SGEMM_OK;
+    if (m > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (!dWscale || !dXscale || !dY || (k && (!dW || !dX))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a matrix or its scales are NULL");
+    if (!aligned(dY, type_bytes(y_type))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "Y is not aligned to its element type");
+    if (!aligned(dWscale, 4) || !aligned(dXscale, 4) || !aligned(dBias, 4))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "scales and bias are FP32 and must be aligned to 4 bytes");
+    LinearPlan p;
+    if ((rc = plan_linear(h, v, dW, dX, m, n, k, ldw, ldx, &p))) return rc;
+    LinearArgs a{dW, dWscale, dX, dXscale, dBias, dY, v.status, m, n, k, ldw, ldx, ldy, (uint32_t)y_type, 0, 0};
+    const uint32_t tile_m = p.index == kLinear ? 256 : p.few ? I8_BM : I8_SIMT_TILE;
+    const uint32_t tile_n = p.index == kLinear ? v.tile_n : p.few ? p.few->tile_n : I8_SIMT_TILE;
+    a.tiles_m = ceil_div(m, tile_m);
+    a.tiles_n = ceil_div(n, tile_n);
+    const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
+    if (tiles * p.parts > 0x7FFFFFFFull) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (p.index == kLinearSimt) {
+        void *params[] = {&a};
+        rc = i8_launch(h, v.functions[kLinearSimt], (uint32_t)tiles, I8_SIMT_THREADS, 0, 0, stream, params);
+        i8_note(h, 2, 1, (uint32_t)tiles, tile_n);
+        return rc;
+    }
+    I8TensorMap map_w, map_x;
+    const uint32_t box_n = p.few ? tile_n : tile_n / 2;
+    if ((rc = i8_encode(h, &map_w, kMapInt8, dW, k, m, ldw, I8_BK, I8_BM, true))) return rc;
+    if ((rc = i8_encode(h, &map_x, kMapInt8, dX, k, n, ldx, I8_BK, box_n, true))) return rc;
+    void *params[] = {&a, &map_w, &map_x};
+    if (p.few) {
+        rc = i8_launch(h, v.functions[p.index], (uint32_t)tiles * p.parts, I8_FEW_THREADS, p.few->smem, p.parts, stream, params);
+        i8_note(h, 3, p.parts, (uint32_t)tiles * p.parts, tile_n);
+        return rc;
+    }
+    const uint32_t grid = kSmsPerPair * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)std::max(1, v.sm_count / (int)kSmsPerPair));
+    rc = i8_launch(h, v.functions[kLinear], grid, v.main_threads, v.main_smem, 0, stream, params);
+    i8_note(h, 1, 1, grid, tile_n);
+    return rc;
+}
+
+SGEMM_API int sgemm_i8_quantize(sgemm_handle *h, const void *dX, int x_type, int8_t *dQ, float *dScale, uint32_t k, uint32_t n,
+                                uint32_t ldx, uint32_t ldq, int pow2, void *stream) {
+    const char *op = "sgemm_i8_quantize";
+    I8View v;
+    int rc = begin(h, op, &v);
+    if (rc) return rc;
+    if (!known_type(x_type)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X's type is FP32 (0), FP16 (1) or BF16 (2)");
+    if (pow2 != 0 && pow2 != 1) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "pow2 is 0 (scale max/127) or 1 (power of two)");
+    if (ldx < std::max(k, 1u) || ldq < std::max(k, 1u))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a leading dimension is smaller than the rows it must hold");
+    if (n == 0) return SGEMM_OK;
+    if (k > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (!dScale || (k && (!dX || !dQ))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X, Q or the scales are NULL");
+    const uint32_t eb = type_bytes(x_type), per = 16 / eb;
+    if (!aligned(dX, eb) || !aligned(dScale, 4)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X or the scales are not aligned to their element type");
+    const bool vec = aligned(dX, 16) && (uint64_t)ldx * eb % 16 == 0 && aligned(dQ, per) && ldq % per == 0;
+    RowArgs a{dX, nullptr, nullptr, nullptr, dQ, dScale, k, n, ldx, 0, 0, ldq, 32, (uint32_t)pow2, 0.0f};
+    return launch_rows(h, v, kQuantize, x_type, vec, a, stream);
+}
+
+SGEMM_API int sgemm_i8_restore(sgemm_handle *h, const int8_t *dQ, const float *dScale, void *dOut, int out_type, uint32_t k,
+                               uint32_t n, uint32_t ldq, uint32_t ldo, void *stream) {
+    const char *op = "sgemm_i8_restore";
+    I8View v;
+    int rc = begin(h, op, &v);
+    if (rc) return rc;
+    if (!known_type(out_type)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "the output's type is FP32 (0), FP16 (1) or BF16 (2)");
+    if (ldq < std::max(k, 1u) || ldo < std::max(k, 1u))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a leading dimension is smaller than the rows it must hold");
+    if (n == 0 || k == 0) return SGEMM_OK;
+    if (k > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (!dQ || !dScale || !dOut) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "Q, the scales or the output are NULL");
+    const uint32_t eb = type_bytes(out_type);
+    if (!aligned(dOut, eb) || !aligned(dScale, 4)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "the output or the scales are not aligned to their element type");
+    const bool vec = aligned(dQ, 16) && ldq % 16 == 0 && aligned(dOut, 16) && (uint64_t)ldo * eb % 16 == 0;
+    const uint64_t units = (uint64_t)(vec ? ceil_div(k, 16) : k) * n;
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>((units + 255) / 256, (uint64_t)v.sm_count * 32);
+    void *params[] = {&dQ, &dScale, &dOut, &k, &n, &ldq, &ldo};
+    return i8_launch(h, v.functions[kRestore + 2 * out_type + (vec ? 0 : 1)], blocks, 256, 0, 0, stream, params);
+}
+
+SGEMM_API int sgemm_i8_rmsnorm(sgemm_handle *h, const void *dX, const void *dResidual, const void *dGamma, int x_type, float eps,
+                               int8_t *dQ, float *dScale, void *dSum, uint32_t k, uint32_t n, uint32_t ldx, uint32_t ldr,
+                               uint32_t ldq, uint32_t lds, void *stream) {
+    const char *op = "sgemm_i8_rmsnorm";
+    I8View v;
+    int rc = begin(h, op, &v);
+    if (rc) return rc;
+    if (!known_type(x_type)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X's type is FP32 (0), FP16 (1) or BF16 (2)");
+    if (!(eps >= 0.0f) || eps > 3.0e38f) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "eps must be a finite number that is not negative");
+    if (k == 0) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "K = 0: the mean of no squares is not defined");
+    if (ldx < k || ldq < k || (dResidual && ldr < k) || (dSum && lds < k))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a leading dimension is smaller than the rows it must hold");
+    if (n == 0) return SGEMM_OK;
+    if (k > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (!dX || !dGamma || !dQ || !dScale) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X, gamma, Q or the scales are NULL");
+    const uint32_t eb = type_bytes(x_type), per = 16 / eb;
+    if (!aligned(dX, eb) || !aligned(dGamma, eb) || !aligned(dResidual, eb) || !aligned(dSum, eb) || !aligned(dScale, 4))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a matrix is not aligned to its element type");
+    if ((dSum == dX && dX && lds != ldx) || (dSum == dResidual && dSum && lds != ldr))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "the sum may replace X or the residual only with the same leading dimension");
+    auto vector_ok = [&](const void *p, uint32_t ld) { return !p || (aligned(p, 16) && (uint64_t)ld * eb % 16 == 0); };
+    const bool vec = vector_ok(dX, ldx) && vector_ok(dResidual, ldr) && vector_ok(dSum, lds) && aligned(dGamma, 16) &&
+                     aligned(dQ, per) && ldq % per == 0;
+    RowArgs a{dX, dResidual, dGamma, dSum, dQ, dScale, k, n, ldx, ldr, lds, ldq, 32, 0, eps};
+    return launch_rows(h, v, kNorm, x_type, vec, a, stream);
+}
+
+SGEMM_API int sgemm_i8_wgrad(sgemm_handle *h, const int8_t *dQ, const float *dScale, const void *dG, int g_type, const void *dC,
+                             void *dD, int d_type, float alpha, float beta, uint32_t m, uint32_t n, uint32_t tokens,
+                             uint32_t ldq, uint32_t ldg, uint32_t ldc, uint32_t ldd, void *stream) {
+    const char *op = "sgemm_i8_wgrad";
+    I8View v;
+    int rc = begin(h, op, &v);
+    if (rc) return rc;
+    if (g_type != (int)SGEMM_I8_FP16 && g_type != (int)SGEMM_I8_BF16) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "G's type is FP16 (1) or BF16 (2)");
+    if (!known_type(d_type)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "D's type is FP32 (0), FP16 (1) or BF16 (2)");
+    if (ldq < std::max(m, 1u) || ldg < std::max(n, 1u) || ldd < std::max(m, 1u) || (beta != 0.0f && ldc < std::max(m, 1u)))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a leading dimension is smaller than the rows it must hold");
+    if (m == 0 || n == 0) return SGEMM_OK;
+    if (m > kLargest || n > kLargest || tokens > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (!dD || (tokens && (!dQ || !dScale || !dG))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "D, the checkpoint, its scales or G are NULL");
+    if (beta != 0.0f && !dC) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "C is NULL but beta != 0");
+    if (beta != 0.0f && dC == dD && ldc != ldd)
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "D may replace C only with the same leading dimension");
+    if (!aligned(dG, 2) || !aligned(dScale, 4) || !aligned(dD, type_bytes(d_type)) || (beta != 0.0f && !aligned(dC, type_bytes(d_type))))
+        return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a matrix is not aligned to its element type");
+    const bool tma = aligned(dQ, 16) && ldq % 16 == 0 && aligned(dG, 16) && ldg % 8 == 0 && tokens > 0;
+    if ((v.force_variant == 1 || v.force_variant == 3) && !tma)
+        return refuse(h, SGEMM_ERR_UNSUPPORTED, op, "the tensor kernel is forced but the operands need 16-byte aligned bases, ldq a multiple of 16, ldg of 8, and a token");
+    WgradArgs a{dQ, dScale, dG, dC, dD, v.status, m, n, tokens, ldq, ldg, ldc, ldd, (uint32_t)g_type, (uint32_t)d_type, alpha, beta, 0, 0};
+    if (!tma || v.force_variant == 2) {
+        a.tiles_m = ceil_div(m, I8_SIMT_TILE);
+        a.tiles_n = ceil_div(n, I8_SIMT_TILE);
+        const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
+        if (tiles > 0x7FFFFFFFull) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+        void *params[] = {&a};
+        rc = i8_launch(h, v.functions[kWgradSimt], (uint32_t)tiles, I8_SIMT_THREADS, 0, 0, stream, params);
+        i8_note(h, 2, 1, (uint32_t)tiles, I8_SIMT_TILE);
+        return rc;
+    }
+    a.tiles_m = ceil_div(m, 256);
+    a.tiles_n = ceil_div(n, 256);
+    const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
+    if (tiles > 0x3FFFFFFFull) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    const uint32_t pairs = (uint32_t)std::max(1, v.sm_count / (int)kSmsPerPair), stages = ceil_div(tokens, I8W_BK);
+    // too few tiles for the device: cut the tokens into 2 or 4 parts that still run at the same time
+    uint32_t parts = 1;
+    while (parts < 4 && tiles * parts * 2 <= pairs && stages >= parts * 8) parts *= 2;
+    if (v.split_k > 0) parts = v.split_k >= 4 ? 4u : v.split_k >= 2 ? 2u : 1u;
+    while (parts > 1 && stages < parts) parts /= 2;
+    const uint32_t units = parts > 1 ? (uint32_t)tiles : (uint32_t)std::min<uint64_t>(tiles, pairs);
+    const uint32_t grid = units * 2 * parts;
+    I8TensorMap map_q, map_g;
+    if ((rc = i8_encode(h, &map_q, kMapInt8, dQ, m, tokens, ldq, 128, I8W_BK, false))) return rc;
+    if ((rc = i8_encode(h, &map_g, g_type == (int)SGEMM_I8_BF16 ? kMapBf16 : kMapFp16, dG, n, tokens, (uint64_t)ldg * 2, 64, I8W_BK, true))) return rc;
+    void *params[] = {&a, &map_q, &map_g};
+    rc = i8_launch(h, v.functions[kWgrad], grid, I8W_THREADS, I8W_SMEM, 2 * parts, stream, params);
+    i8_note(h, 1, parts, grid, 256);
+    return rc;
+}

@@ -1,0 +1,41 @@
+// Constants of the 8-bit kernels that the device code (text-included by the generator) and the host planner
+// (sgemm_i8.cpp) have to agree on.  Preprocessor definitions only.
+#ifndef SGEMM_I8_PARAMS_HPP
+#define SGEMM_I8_PARAMS_HPP
+
+// element type codes of the entry points (the generator's DataType numbers)
+#define SGEMM_I8_FP32 0u
+#define SGEMM_I8_FP16 1u
+#define SGEMM_I8_BF16 2u
+
+// ---- linear: k per stage (one 128-byte swizzle span of int8), rows of W per CTA
+#define I8_BK 128
+#define I8_BM 128
+// few-token kernels: tile 128 channels x TN tokens, one tile and one K range per CTA, the CTAs of a cluster share a tile
+#define I8_FEW_THREADS 128
+#define I8_FEW_SMEM(tn, stages) ((stages) * (I8_BM + (tn)) * I8_BK + 1024 + 256)
+#define I8_FEW_STAGES_16 6
+#define I8_FEW_STAGES_32 5
+#define I8_FEW_STAGES_64 4
+#define I8_FEW_STAGES_128 6
+// largest K whose integer sum cannot leave 32 bits: K * 128 * 128 < 2^31
+#define I8_MAX_K 131071u
+
+// ---- fallback kernels for operands TMA cannot describe: square tiles
+#define I8_SIMT_TILE 64
+#define I8_SIMT_THREADS 256
+
+// ---- weight gradient: 256 x 256 tile per CTA pair, tokens per stage
+#define I8W_BK 64
+#define I8W_STAGES 5
+#define I8W_THREADS 512
+#define I8W_STAGE_BYTES (128 * I8W_BK + 2 * 128 * I8W_BK + 2 * 128 * I8W_BK)
+#define I8W_SMEM (I8W_STAGES * I8W_STAGE_BYTES + 1024 + 256)
+#define I8W_LAUNCH_REGS 128   // what 512 threads leave per thread; the register hand-over below starts from it
+#define I8W_CHAIN 8           // stages accumulated inside the tensor core before the sum moves to FP32 registers
+
+// ---- row kernels: 16-byte vectors of the input one thread keeps in registers
+#define I8_ROW_THREADS 256
+#define I8_ROW_MAX_THREADS 1024
+
+#endif

@@ -51,4 +51,36 @@ int launch_with_scratch(sgemm_handle *h, void *scratch, size_t scratch_bytes, co
                         const float *dC, float *dD, float alpha, float beta, uint32_t m, uint32_t n, uint32_t k,
                         uint32_t lda, uint32_t ldb, uint32_t ldc, uint32_t ldd, void *stream);
 
+// ---- seam of the 8-bit entry points (sgemm_i8.cpp) ----------------------------------------------------------------
+// A CUDA tensor map as plain bytes (the host code of the entry points needs no <cuda.h>).
+struct alignas(64) I8TensorMap {
+    uint64_t opaque[16];
+};
+constexpr int kI8Functions = 48;
+// What the planner needs to know about a handle of an INT8 cubin.
+struct I8View {
+    void *const *functions = nullptr;   // kernels by index (sgemm_i8.cpp numbers and names them)
+    uint32_t *status = nullptr;         // device status words
+    int sm_count = 0;
+    uint32_t tile_n = 0, main_threads = 0, main_smem = 0;   // the main linear kernel as generated
+    int64_t force_variant = 0, split_k = 0;                 // options of sgemm_set_option
+};
+// False when the handle's cubin was not generated for INT8 operands.
+bool i8_view(sgemm_handle *h, I8View *view);
+// The kernels sgemm_open resolves in an INT8 cubin: their names, the dynamic shared memory they opt in to, and, where a
+// kernel hands registers from one warp group to another, the registers per thread it must have been compiled to (else 0).
+int i8_function_count();
+const char *i8_function_name(int index);
+uint32_t i8_function_smem(int index, uint32_t main_smem);
+int i8_function_registers(int index);
+// Launch on the handle's context; cluster: CTAs per cluster (0: as compiled).
+int i8_launch(sgemm_handle *h, void *function, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, void *stream,
+              void **params);
+// 2-D tensor map, dims {d0 (contiguous), d1}, box {b0, b1}, with the 128-byte swizzle or none.
+enum I8MapType { kMapInt8, kMapFp16, kMapBf16 };
+int i8_encode(sgemm_handle *h, I8TensorMap *map, I8MapType type, const void *base, uint64_t d0, uint64_t d1, uint64_t stride_bytes,
+              uint32_t b0, uint32_t b1, bool swizzle);
+// What sgemm_get_info reports as "last_variant", "last_split_k", "last_grid" and "last_tile_n".
+void i8_note(sgemm_handle *h, int variant, uint32_t parts, uint32_t grid, uint32_t tile_n);
+
 }  // namespace sgemm_internal

@@ -115,7 +115,8 @@ struct sgemm_handle {
     CUdevice cu_device = 0;
     CUcontext ctx = nullptr;
     CUmodule module = nullptr;
-    uint32_t elem_bytes = 4;    // size of an element of A and B: 4 (FP32) or 2 (FP16 / BF16, tensor variant only)
+    uint32_t elem_bytes = 4;    // size of an element of A and B: 4 (FP32), 2 (FP16 / BF16) or 1 (INT8), the latter two tensor variant only
+    void *i8_functions[sgemm_internal::kI8Functions] = {};   // INT8 cubins: the kernels of the 8-bit entry points
     CUfunction fn_pack16 = nullptr, fn_repitch = nullptr, fn_narrow16 = nullptr;
     CUfunction fn_main = nullptr, fn_simt = nullptr, fn_split_lo = nullptr, fn_pack_a = nullptr,
                fn_reduce = nullptr, fn_fill = nullptr, fn_tile_map = nullptr, fn_wait_selftest = nullptr;
@@ -202,6 +203,11 @@ struct CtxGuard {
     }
 };
 
+// the FP32-result calls on a handle of an INT8 cubin
+int refuse_i8(sgemm_handle *h) {
+    return fail(h, SGEMM_ERR_UNSUPPORTED, "this cubin is for INT8 operands with scales: use the sgemm_i8_* entry points");
+}
+
 size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // ------------------------------------------------------------------------------------ launch plan
@@ -265,6 +271,7 @@ uint32_t pick_split_k(const sgemm_handle *h, uint32_t tiles, uint32_t k, uint32_
 
 int make_plan(sgemm_handle *h, const void *a, const void *b, uint32_t m, uint32_t n, uint32_t k, uint32_t lda,
               uint32_t ldb, Plan *p) {
+    if (h->elem_bytes == 1) return refuse_i8(h);
     bool eligible = tensor_eligible(h, a, b, lda, ldb);
     p->lda_eff = lda;
     p->ldb_eff = ldb;
@@ -444,22 +451,31 @@ int encode_map(sgemm_handle *h, int slot, const void *base, uint64_t d0, uint64_
 }
 
 int launch(sgemm_handle *h, CUfunction f, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bx, uint32_t by,
-           uint32_t smem, CUstream s, void **params) {
-    if (h->pdl) {
+           uint32_t smem, CUstream s, void **params, uint32_t cluster = 0 /* CTAs per cluster; 0: as the kernel was compiled */) {
+    if (h->pdl || cluster) {
         // programmatic dependent launch: the kernel may be scheduled while its predecessor in the stream is still
         // running; every kernel of the cubin executes griddepcontrol.wait before it touches global memory, so
         // only launch latency and per-CTA set-up overlap with the predecessor, never data.
-        CUlaunchAttribute attr;
-        attr.id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
-        attr.value.programmaticStreamSerializationAllowed = 1;
+        CUlaunchAttribute attrs[2];
+        uint32_t count = 0;
+        if (h->pdl) {
+            attrs[count].id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
+            attrs[count++].value.programmaticStreamSerializationAllowed = 1;
+        }
+        if (cluster) {
+            attrs[count].id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+            attrs[count].value.clusterDim.x = cluster;
+            attrs[count].value.clusterDim.y = 1;
+            attrs[count++].value.clusterDim.z = 1;
+        }
         CUlaunchConfig cfg;
         std::memset(&cfg, 0, sizeof cfg);
         cfg.gridDimX = gx; cfg.gridDimY = gy; cfg.gridDimZ = gz;
         cfg.blockDimX = bx; cfg.blockDimY = by; cfg.blockDimZ = 1;
         cfg.sharedMemBytes = smem;
         cfg.hStream = s;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
+        cfg.attrs = attrs;
+        cfg.numAttrs = count;
         CU_CHECK(h, driver().cuLaunchKernelEx_(&cfg, f, params, nullptr));
     } else {
         CU_CHECK(h, driver().cuLaunchKernel_(f, gx, gy, gz, bx, by, 1, smem, s, params, nullptr));
@@ -493,6 +509,7 @@ int launch_main(sgemm_handle *h, CUfunction f, uint32_t gx, uint32_t gz, uint32_
 int check_problem(sgemm_handle *h, const void *a, const void *b, const void *c, const void *d, float beta,
                   uint32_t m, uint32_t n, uint32_t k, uint32_t lda, uint32_t ldb, uint32_t ldc, uint32_t ldd) {
     if (!h) return SGEMM_ERR_INVALID_ARGUMENT;
+    if (h->elem_bytes == 1) return refuse_i8(h);
     if (m && n && !d) return fail(h, SGEMM_ERR_INVALID_ARGUMENT, "D is NULL");
     if (m && n && k && (!a || !b)) return fail(h, SGEMM_ERR_INVALID_ARGUMENT, "A or B is NULL");
     if (m && n && beta != 0.0f && !c) return fail(h, SGEMM_ERR_INVALID_ARGUMENT, "C is NULL but beta != 0");
@@ -840,14 +857,14 @@ SGEMM_API int sgemm_open(const char *cubin_path, const char *toml_path, int devi
     sgemm_handle *h = new sgemm_handle();
     h->cfg = cfg;
     h->device = device;
-    // element types as the generator numbers them: 0 = FP32, 1 = FP16, 2 = BF16
-    if (cfg.a_type != cfg.b_type || cfg.a_type < 0 || cfg.a_type > 2 || cfg.cd_type != 0 || cfg.scalar_type != 0 ||
+    // element types as the generator numbers them: 0 = FP32, 1 = FP16, 2 = BF16, 3 = INT8
+    if (cfg.a_type != cfg.b_type || cfg.a_type < 0 || cfg.a_type > 3 || cfg.cd_type != 0 || cfg.scalar_type != 0 ||
         (cfg.a_type != 0 && cfg.variant != kVariantTensor)) {
         delete h;
         return fail(nullptr, SGEMM_ERR_UNSUPPORTED, "element types a %d b %d cd %d scalar %d are not served (FP32 everywhere, or "
-                    "FP16/BF16 A and B with the tensor variant)", cfg.a_type, cfg.b_type, cfg.cd_type, cfg.scalar_type);
+                    "FP16/BF16/INT8 A and B with the tensor variant)", cfg.a_type, cfg.b_type, cfg.cd_type, cfg.scalar_type);
     }
-    h->elem_bytes = cfg.a_type == 0 ? 4u : 2u;
+    h->elem_bytes = cfg.a_type == 0 ? 4u : cfg.a_type == 3 ? 1u : 2u;
     sgemm_config_tile(&cfg, &h->tile_m, &h->tile_n);
     auto bail = [&](int code) {
         g_open_error = h->error;
@@ -961,6 +978,27 @@ SGEMM_API int sgemm_open(const char *cubin_path, const char *toml_path, int devi
             fail(h, SGEMM_ERR_MODULE, "'%s' in '%s' uses %d registers per thread where its register hand-over assumes %d",
                  e.name, cubin_path, regs, expect);
             return bail(SGEMM_ERR_MODULE);
+        }
+    }
+    if (h->elem_bytes == 1) {   // the kernels of the 8-bit entry points
+        for (int i = 0; i < sgemm_internal::i8_function_count(); ++i) {
+            const char *name = sgemm_internal::i8_function_name(i);
+            CUfunction fn = nullptr;
+            const uint32_t smem = sgemm_internal::i8_function_smem(i, (uint32_t)cfg.dynamic_smem_bytes);
+            const int expect = sgemm_internal::i8_function_registers(i);
+            int regs = 0;
+            if ((r = d.cuModuleGetFunction_(&fn, h->module, name)) != CUDA_SUCCESS ||
+                (smem && (r = d.cuFuncSetAttribute_(fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)smem)) != CUDA_SUCCESS) ||
+                (expect && (r = d.cuFuncGetAttribute_(&regs, CU_FUNC_ATTRIBUTE_NUM_REGS, fn)) != CUDA_SUCCESS)) {
+                fail(h, SGEMM_ERR_MODULE, "entry point '%s' unusable in '%s': %s", name, cubin_path, cu_text(r).c_str());
+                return bail(SGEMM_ERR_MODULE);
+            }
+            if (regs != expect) {
+                fail(h, SGEMM_ERR_MODULE, "'%s' in '%s' uses %d registers per thread where its register hand-over assumes %d",
+                     name, cubin_path, regs, expect);
+                return bail(SGEMM_ERR_MODULE);
+            }
+            h->i8_functions[i] = reinterpret_cast<void *>(fn);
         }
     }
     if ((r = d.cuMemAlloc_(&h->status, kStatusAlloc * 4)) != CUDA_SUCCESS ||
@@ -1450,6 +1488,51 @@ int with_context(sgemm_handle *h, int (*fn)(void *), void *arg) {
 void **noalloc_scratch_slot(sgemm_handle *h) { return h ? &h->noalloc_scratch : nullptr; }
 
 CommState *comm_state(sgemm_handle *h) { return h ? &h->comm : nullptr; }
+
+bool i8_view(sgemm_handle *h, I8View *view) {
+    if (h->elem_bytes != 1) return false;
+    view->functions = h->i8_functions;
+    view->status = reinterpret_cast<uint32_t *>(h->status);
+    view->sm_count = h->sm_count;
+    view->tile_n = h->tile_n;
+    view->main_threads = (uint32_t)h->cfg.num_threads;
+    view->main_smem = (uint32_t)h->cfg.dynamic_smem_bytes;
+    view->force_variant = h->force_variant;
+    view->split_k = h->split_k_opt;
+    return true;
+}
+
+int i8_launch(sgemm_handle *h, void *function, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, void *stream,
+              void **params) {
+    CtxGuard guard(h);
+    return launch(h, reinterpret_cast<CUfunction>(function), grid, 1, 1, threads, 1, smem, (CUstream)stream, params, cluster);
+}
+
+int i8_encode(sgemm_handle *h, I8TensorMap *map, I8MapType type, const void *base, uint64_t d0, uint64_t d1, uint64_t stride_bytes,
+              uint32_t b0, uint32_t b1, bool swizzle) {
+    static_assert(sizeof(I8TensorMap) == sizeof(CUtensorMap) && alignof(I8TensorMap) >= alignof(CUtensorMap), "a tensor map's bytes");
+    const CUtensorMapDataType dtype = type == kMapInt8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                      : type == kMapFp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t dims[2] = {d0, d1}, strides[1] = {stride_bytes};
+    const cuuint32_t box[2] = {b0, b1}, estr[2] = {1, 1};
+    CUresult r = driver().cuTensorMapEncodeTiled_(reinterpret_cast<CUtensorMap *>(map), dtype, 2, const_cast<void *>(base), dims, strides,
+                                                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(h, SGEMM_ERR_CUDA, "cuTensorMapEncodeTiled(base %p, dims %llu x %llu, pitch %llu, box %u x %u) -> %s", base,
+                    (unsigned long long)d0, (unsigned long long)d1, (unsigned long long)stride_bytes, b0, b1, cu_text(r).c_str());
+    return SGEMM_OK;
+}
+
+void i8_note(sgemm_handle *h, int variant, uint32_t parts, uint32_t grid, uint32_t tile_n) {
+    h->last_variant = variant;
+    h->last_split_k = parts;
+    h->last_grid = grid;
+    h->last_tile_n = tile_n;
+    h->last_feed_tma = variant != 2;
+    h->last_acc_chain = 0;
+}
 
 int launch_with_scratch(sgemm_handle *h, void *scratch, size_t scratch_bytes, const float *dA, const float *dB,
                         const float *dC, float *dD, float alpha, float beta, uint32_t m, uint32_t n, uint32_t k,

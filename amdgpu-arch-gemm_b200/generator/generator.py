@@ -20,7 +20,8 @@ How the reference's knobs are read on sm_100a
 ---------------------------------------------
 ``mfma = (M, N, B, K)`` is the MMA atom.  ``(128, N, 1, 8)`` selects the tensor-core variant
 (tcgen05 ``kind::tf32``, one CTA issues 128 x N x 8; with FP16 / BF16 operands the atom is
-``(128, N, 1, 16)``, tcgen05 ``kind::f16``); ``(1, 1, 1, 1)`` selects the FFMA SIMT variant.
+``(128, N, 1, 16)``, tcgen05 ``kind::f16``, with INT8 ``(128, N, 1, 32)``, tcgen05 ``kind::i8``);
+``(1, 1, 1, 1)`` selects the FFMA SIMT variant.
 The GCN shapes ``(16,16,1,4)`` / ``(32,32,1,2)`` of the reference's tuner are still accepted: they have
 no tensor-core counterpart for FP32 operands, so they map to the SIMT variant with the same block tile.
 ``wave_group`` is the cluster shape for the tensor variant and the thread grid of a block for SIMT;
@@ -116,10 +117,12 @@ def gpu_function(func):
 class DataType(IntEnum):
     """Element types.  The reference has FP32 only (generator/generator.py:816-824) and plumbs ``a_type`` ...
     ``scalar_type`` to its TOML as these integers; FP16 and BF16 are additions for the A and B operands of the
-    tensor variant (C, D and the scalars stay FP32)."""
+    tensor variant (C, D and the scalars stay FP32), and so is INT8: operands in 8 bits with one FP32 scale per row of
+    op(A) and column of B, served by the ``sgemm_i8_*`` entry points of the runner."""
     FP32 = 0
     FP16 = 1
     BF16 = 2
+    INT8 = 3
 
 
 def datatype_size(dtype: DataType) -> int:
@@ -127,6 +130,8 @@ def datatype_size(dtype: DataType) -> int:
         return 4
     if dtype in (DataType.FP16, DataType.BF16):
         return 2
+    if dtype == DataType.INT8:
+        return 1
     raise RuntimeError(f"unrecognized type {dtype}")
 
 
@@ -230,7 +235,7 @@ class GemmSolutionConfig:
             raise RuntimeError("tiling parameters must be positive")
 
         m0 = self.mfma[0]
-        if m0 == 128 and self.mfma[3] == (8 if self.elem_bytes == 4 else 16):
+        if m0 == 128 and self.mfma[3] == 32 // self.elem_bytes:   # 32 bytes of K per operand row
             self.variant = VARIANT_TENSOR
             self._check_tensor()
         elif self.mfma == (1, 1, 1, 1) or self.mfma in ((16, 16, 1, 4), (32, 32, 1, 2)):
@@ -238,7 +243,7 @@ class GemmSolutionConfig:
             self._check_simt()
         else:
             raise RuntimeError(f"unsupported MMA atom {self.mfma}: use (128, N, 1, 8) for tcgen05 tf32 (FP32 operands), "
-                               f"(128, N, 1, 16) for tcgen05 f16/bf16, "
+                               f"(128, N, 1, 16) for tcgen05 f16/bf16, (128, N, 1, 32) for tcgen05 i8, "
                                f"(1, 1, 1, 1) for FFMA, or a legacy (16,16,1,4)/(32,32,1,2) shape")
 
         if self.variant == VARIANT_TENSOR and self.feed != "ldg":
@@ -249,6 +254,21 @@ class GemmSolutionConfig:
 
     # ------------------------------------------------------------------ variant-specific checks
     def _check_tensor(self):
+        if self.elem_bytes == 1:
+            # INT8 operands: integer sums are exact, so there are no lo terms and no accumulation chains; both operands
+            # are K-contiguous (A transposed, B not), the layout of weights and activations; the cubin carries the
+            # kernels for few tokens, for 8-bit rows and for the weight gradient beside the main one
+            if not self.trans_a or self.trans_b:
+                raise RuntimeError("INT8 operands are read K-contiguous: trans_a=True, trans_b=False")
+            if self.wave_group != (2, 1):
+                raise RuntimeError("INT8 operands run on CTA pairs: wave_group (2, 1)")
+            if self.depth_k != 128:
+                raise RuntimeError(f"depth_k = {self.depth_k} must be 128 (one 128-byte span of int8)")
+            if self.split != "prepass" or self.a_major != "mn":
+                raise RuntimeError("split and a_major do not apply to INT8 operands")
+            if self.acc_chain or self.epilogue_warps not in (None, 8):
+                raise RuntimeError("INT8 operands take no acc_chain and 8 epilogue warps")
+            self.terms, self.companion, self.acc_chain = 1, False, 0
         if self.elem_bytes == 2:
             # FP16 / BF16 operands: one kind::f16 MMA per 16 k (no split).  Every operand is read where it lies: stored
             # K-contiguous (A transposed, B untransposed) as a K-major tile, stored M- or N-contiguous as an MN-major
@@ -559,6 +579,10 @@ def _tensor_defines(config: GemmSolutionConfig):
             ("TC_ACC_CHUNK", config.acc_chain // config.depth_k)]
 
 
+def _i8_defines(config: GemmSolutionConfig):
+    return [("I8_BN", config.tile_size[1]), ("I8_STAGES", config.stages)]
+
+
 def _trans_defines(cfg: GemmSolutionConfig):
     return [("GEMM_TRANS_A", 1 if cfg.trans_a else 0), ("GEMM_TRANS_B", 1 if cfg.trans_b else 0)]
 
@@ -587,7 +611,13 @@ def gemm(context: GpuContext, name: str, arch: str, config: GemmSolutionConfig, 
               f"wgm {opt.wgm}, plr {opt.plr}, gw {opt.gw}\n")
     out.write(_defines([("OPT_WGM", opt.wgm)] + _trans_defines(config)))
     out.write(_read("sgemm_common.cuh"))
-    if config.variant == VARIANT_SIMT and config.feed == "tma":
+    if config.elem_bytes == 1:
+        # the 8-bit operators: main linear kernel under the entry name with its few-token and fallback siblings, the row
+        # kernels that make and undo 8-bit rows, the weight gradient
+        out.write(_defines(_i8_defines(config)))
+        for part in ("sgemm_i8_params.hpp", "sgemm_i8_common.cuh", "sgemm_i8_rows.cuh", "sgemm_i8_linear.cuh", "sgemm_i8_wgrad.cuh"):
+            out.write(_read(part))
+    elif config.variant == VARIANT_SIMT and config.feed == "tma":
         # the register-fed kernel under the fallback name (as in a tensor-variant cubin), the TMA-fed one as the entry
         out.write(_defines(_simt_defines(simt_fallback_config(config.trans_a, config.trans_b), opt, SIMT_FALLBACK_ENTRY)))
         out.write(_read("sgemm_simt.cuh"))
@@ -685,8 +715,8 @@ def compile(kern_name: str, kern_str: str, arch: str, output_folder: str, gemm_c
 def tensor_config(bn: int = 256, bk: int = 32, stages: int = 2, cluster: int = 1, trans_a: bool = False,
                   trans_b: bool = False, ab_type: DataType = DataType.FP32, **kw) -> GemmSolutionConfig:
     """Shorthand for a tensor-variant configuration with tile (128 * cluster) x bn x bk; ``ab_type`` is the element
-    type of A and B (FP32: 3xTF32 with atom K = 8; FP16 / BF16: one MMA per 16 k)."""
-    atom_k = 8 if ab_type == DataType.FP32 else 16
+    type of A and B (FP32: 3xTF32 with atom K = 8; FP16 / BF16: one MMA per 16 k; INT8: one per 32 k)."""
+    atom_k = 32 // datatype_size(ab_type)
     return GemmSolutionConfig(ab_type, ab_type, DataType.FP32, DataType.FP32,
                               (128, bn, 1, atom_k), (cluster, 1), (1, 1), bk, trans_a, trans_b, vmem_stage=stages - 1, **kw)
 

@@ -66,6 +66,8 @@ REGISTRY = {
     "fp16_tc2_256x128x64_s4_tn": (lambda: tensor_config(128, 64, 4, cluster=2, trans_a=True, ab_type=DataType.FP16), dict(wgm=8)),
     "bf16_tc2_256x256x64_s6_tt": (lambda: tensor_config(256, 64, 6, cluster=2, trans_a=True, trans_b=True, ab_type=DataType.BF16), dict(wgm=8)),
     "fp16_tc_128x128x64_s4_nt": (lambda: tensor_config(128, 64, 4, trans_b=True, ab_type=DataType.FP16), dict(wgm=8)),
+    # INT8 operands with scales (the sgemm_i8_* entry points): linear layer, 8-bit rows, weight gradient
+    "i8_tc2_256x256x128_s6": (lambda: tensor_config(256, 128, 6, cluster=2, trans_a=True, ab_type=DataType.INT8), dict(wgm=8)),
     "simt_128x128x16": (lambda: simt_config(128, 128, 16, 8, 8), dict(wgm=8)),
     "simt_128x128x16_t16x8": (lambda: simt_config(128, 128, 16, 16, 8), dict(wgm=8)),   # best of the FFMA sweep at 4096^3
     "simt_64x64x16": (lambda: simt_config(64, 64, 16, 4, 4), dict(wgm=4)),
@@ -84,6 +86,7 @@ REGISTRY = {
 
 DEFAULT_TENSOR = "tc2_256x256x32_s3"
 DEFAULT_SIMT = "simt_128x128x16"
+DEFAULT_I8 = "i8_tc2_256x256x128_s6"
 
 
 def paths(name: str) -> Tuple[str, str]:
@@ -170,7 +173,8 @@ DEFAULT_SIMT_LARGE = "ffma_tma_256x128x32_s3"   # strict FP32 on problems of man
 
 
 def recommend(m: int, n: int, k: int, operands: str = "fp32", strict_fp32: bool = False) -> str:
-    """Registered kernel to use for a problem of this shape on a B200 (NN layout).
+    """Registered kernel to use for a problem of this shape on a B200 (NN layout; INT8: both operands K-contiguous,
+    one cubin serves every shape, its entry points choose the kernel).
 
     ``strict_fp32`` asks for the FFMA variant (every product and sum in IEEE FP32, what ``force_variant`` 2 runs): the
     tuner table's FFMA entry nearest to the problem if a registered kernel has its structure, else the TMA-fed kernel
@@ -209,6 +213,8 @@ def recommend(m: int, n: int, k: int, operands: str = "fp32", strict_fp32: bool 
         if name is not None:
             return name
         return DEFAULT_SIMT_LARGE if -(-m // 256) * -(-n // 128) >= 2 * 148 else DEFAULT_SIMT
+    if operands == "int8":
+        return DEFAULT_I8
     if operands == "fp32":
         if flops < 2 ** 27:
             return DEFAULT_SIMT

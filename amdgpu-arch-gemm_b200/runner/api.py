@@ -79,6 +79,11 @@ ABI = {
     "sgemm_set_workspace": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t]),
     "sgemm_fill_uniform": (ctypes.c_int, [_vp, _vp, _u64, _u64, _u64, _vp]),
     "sgemm_narrow16": (ctypes.c_int, [_vp, _vp, _vp, _u64, _vp]),
+    "sgemm_i8_linear": (ctypes.c_int, [_vp] * 7 + [ctypes.c_int] + [_u32] * 6 + [_vp]),
+    "sgemm_i8_quantize": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _u32, _u32, _u32, _u32, ctypes.c_int, _vp]),
+    "sgemm_i8_restore": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, _u32, _u32, _u32, _u32, _vp]),
+    "sgemm_i8_rmsnorm": (ctypes.c_int, [_vp] * 4 + [ctypes.c_int, ctypes.c_float, _vp, _vp, _vp] + [_u32] * 6 + [_vp]),
+    "sgemm_i8_wgrad": (ctypes.c_int, [_vp] * 4 + [ctypes.c_int, _vp, _vp, ctypes.c_int, ctypes.c_float, ctypes.c_float] + [_u32] * 7 + [_vp]),
     "sgemm_tile_map": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int32), _u32, _u32]),
     "sgemm_dev_alloc": (ctypes.c_int, [_vp, ctypes.c_size_t, ctypes.POINTER(_vp)]),
     "sgemm_dev_free": (ctypes.c_int, [_vp, _vp]),
@@ -144,6 +149,20 @@ def _ptr(x) -> int:
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)}")
+
+
+_TYPE_CODES = {"float32": 0, "float16": 1, "bfloat16": 2}
+
+
+def _type_code(x, given: Optional[int]) -> int:
+    """Element type of a matrix as the C ABI numbers it (0 FP32, 1 FP16, 2 BF16): the one given, else the tensor's or
+    array's own."""
+    if given is not None:
+        return int(given)
+    name = str(getattr(x, "dtype", "")).replace("torch.", "")
+    if name not in _TYPE_CODES:
+        raise TypeError(f"element type {name or type(x).__name__!r}: pass a FP32, FP16 or BF16 tensor, or the type with an address")
+    return _TYPE_CODES[name]
 
 
 class SgemmRunner:
@@ -213,6 +232,64 @@ class SgemmRunner:
         lda, ldb, ldc, ldd = self._lds(m, n_local, k, lda, ldb, ldc, ldd)
         self._check(self._L.sgemm_run_host_sharded(self._h, _ptr(a), _ptr(b), _ptr(c), _ptr(d), alpha, beta, m, n_local, k,
                                                    lda, ldb, ldc, ldd), "sgemm_run_host_sharded")
+
+    # ------------------------------------------------- 8-bit operands (cubins generated for INT8)
+    def _addr(self, x, name: str, dtype: Optional[str] = None) -> int:
+        """Address of an operand of an 8-bit call; a tensor must lie on the handle's GPU, have the element type the
+        call takes, and hold the elements of a row one after the other."""
+        if x is None or isinstance(x, int) or not hasattr(x, "data_ptr"):
+            return _ptr(x)
+        if not x.is_cuda or x.get_device() != self.device:
+            raise ValueError(f"{name} lies on {x.device}, the handle on GPU {self.device}")
+        if dtype is not None and str(x.dtype) != "torch." + dtype:
+            raise TypeError(f"{name} is {x.dtype}, the call takes {dtype}")
+        if x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise ValueError(f"{name}: the elements of a row must be contiguous")
+        return x.data_ptr()
+
+    def i8_linear(self, w, w_scale, x, x_scale, y, m, n, k, bias=None, ldw=0, ldx=0, ldy=0, y_type=None, stream=0):
+        """Y[i, j] = (sum_k W[k, i] X[k, j]) * x_scale[j] * w_scale[i] (+ bias[i]): ``m`` channels, ``n`` tokens, ``k``
+        features; int8 W and X column-major K x M and K x N (a channel's weights, a token's features contiguous), Y
+        column-major M x N in FP32, FP16 or BF16, scales and bias FP32."""
+        self._check(self._L.sgemm_i8_linear(
+            self._h, self._addr(w, "w", "int8"), self._addr(w_scale, "w_scale", "float32"), self._addr(x, "x", "int8"),
+            self._addr(x_scale, "x_scale", "float32"), self._addr(bias, "bias", "float32"), self._addr(y, "y"),
+            _type_code(y, y_type), m, n, k, ldw or max(k, 1), ldx or max(k, 1), ldy or max(m, 1), stream), "sgemm_i8_linear")
+
+    def i8_quantize(self, x, q, scale, k, n, pow2=False, ldx=0, ldq=0, x_type=None, stream=0):
+        """8-bit columns of the K x N matrix X with one scale each (a token's features or a channel's weights per column):
+        scale max|x|/127, or with ``pow2`` the least power of two that holds the column (activation checkpoints)."""
+        self._check(self._L.sgemm_i8_quantize(
+            self._h, self._addr(x, "x"), _type_code(x, x_type), self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"),
+            k, n, ldx or max(k, 1), ldq or max(k, 1), 1 if pow2 else 0, stream), "sgemm_i8_quantize")
+
+    def i8_restore(self, q, scale, out, k, n, ldq=0, ldo=0, out_type=None, stream=0):
+        """The values ``scale[j] * q[:, j]``, rounded to the output's type."""
+        self._check(self._L.sgemm_i8_restore(
+            self._h, self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"), self._addr(out, "out"),
+            _type_code(out, out_type), k, n, ldq or max(k, 1), ldo or max(k, 1), stream), "sgemm_i8_restore")
+
+    def i8_rmsnorm(self, x, gamma, q, scale, k, n, residual=None, sum_out=None, eps=1e-6, ldx=0, ldr=0, ldq=0, lds=0,
+                   x_type=None, stream=0):
+        """Root-mean-square norm of X (+ residual) times gamma, as 8-bit columns with one scale each; ``sum_out`` receives
+        X + residual in X's type (it may be the residual or X itself)."""
+        code = _type_code(x, x_type)
+        dtype = None if x_type is not None else str(getattr(x, "dtype", "")).replace("torch.", "")
+        self._check(self._L.sgemm_i8_rmsnorm(
+            self._h, self._addr(x, "x"), self._addr(residual, "residual", dtype), self._addr(gamma, "gamma", dtype),
+            code, eps, self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"),
+            self._addr(sum_out, "sum_out", dtype), k, n, ldx or k, ldr or k, ldq or k, lds or k, stream), "sgemm_i8_rmsnorm")
+
+    def i8_wgrad(self, q, scale, dy, dw, m, n, tokens, c=None, alpha=1.0, beta=0.0, ldq=0, lddy=0, ldc=0, lddw=0,
+                 dy_type=None, dw_type=None, stream=0):
+        """Weight gradient from an 8-bit checkpoint: dW[i, j] = alpha * sum_t V(q[i, t], scale[t]) * dY[j, t] + beta * C[i, j] with
+        ``m`` features, ``n`` channels; V is the value ``i8_restore`` gives in dY's type (FP16 or BF16); C and dW have one type."""
+        code = _type_code(dw, dw_type)
+        dtype = None if dw_type is not None else str(getattr(dw, "dtype", "")).replace("torch.", "")
+        self._check(self._L.sgemm_i8_wgrad(
+            self._h, self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"), self._addr(dy, "dy"), _type_code(dy, dy_type),
+            self._addr(c, "c", dtype), self._addr(dw, "dw"), code, alpha, beta, m, n, tokens,
+            ldq or max(m, 1), lddy or max(n, 1), ldc or max(m, 1), lddw or max(m, 1), stream), "sgemm_i8_wgrad")
 
     # ------------------------------------------------------------------------------- multi-GPU
     def comm_init(self, comm_id: bytes, rank: int, world: int):

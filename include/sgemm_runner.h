@@ -265,6 +265,57 @@ int sgemm_fill_uniform(sgemm_handle *h, float *dptr, uint64_t count, uint64_t fi
  * the loaded cubin (FP16 or BF16, round to nearest even); SGEMM_ERR_UNSUPPORTED on an FP32 cubin. */
 int sgemm_narrow16(sgemm_handle *h, const float *dsrc, void *ddst, uint64_t count, void *stream);
 
+/* ---- 8-bit operands -----------------------------------------------------------------------------------------------
+ * No counterpart in the reference (FP32 only).  The calls below need a handle of a cubin generated for INT8 operands
+ * (a_type 3 in its TOML; the FP32-result calls above refuse such a handle).  An 8-bit matrix is a column-major K x N matrix of
+ * int8, leading dimension >= K, with one FP32 scale per column: column j stands for scale[j] * q[:, j].  A column is a
+ * token's features or an output channel's weights.  Element types are 0 = FP32, 1 = FP16, 2 = BF16.
+ *
+ * Every call is asynchronous on `stream`, is one kernel launch, needs no workspace and keeps nothing between calls: calls on
+ * several streams and captured graphs of them need no ordering beyond that of their data.  Any base and leading dimension
+ * is served; 8-bit matrices whose base and leading dimension are multiples of 16 bytes (and G likewise) run on the
+ * tensor cores, others on slower kernels.  Outputs must not overlap inputs except where a call says so; elements between
+ * a column's K and its leading dimension are neither read nor written.  Options "force_variant" (0 auto, 1 tensor main
+ * kernel, 2 fallback, 3 tensor few-token kernel) and "split_k" (parts of the sum, rounded down to 1, 2, 4 or 8) apply;
+ * "last_variant", "last_split_k", "last_grid" and "last_tile_n" tell what sgemm_i8_linear and sgemm_i8_wgrad ran. */
+
+/* Linear layer: Y[i, j] = fp32(sum_k W[k, i] * X[k, j]) * x_scale[j] * w_scale[i] (+ bias[i]) for M channels and N tokens, W
+ * K x M, X K x N, Y M x N (ldy >= M) in y_type, rounded once.  bias: M FP32 values or NULL.  The integer sum is exact
+ * (K <= 131071, larger is SGEMM_ERR_INVALID_ARGUMENT), so results do not depend on tiles or cuts. */
+int sgemm_i8_linear(sgemm_handle *h, const int8_t *dW, const float *dWscale, const int8_t *dX, const float *dXscale,
+                    const float *dBias, void *dY, int y_type, uint32_t m, uint32_t n, uint32_t k,
+                    uint32_t ldw, uint32_t ldx, uint32_t ldy, void *stream);
+
+/* 8-bit columns of X (K x N in x_type) with their scales.  With P = max |x| of a column: pow2 0 gives scale P / 127 and
+ * q = round(127 x / P); pow2 1 gives the least power of two with 127 * scale >= P (at least 2^-126) and q = round(x / scale),
+ * so that scale * q is exact in FP16 and BF16 too (within their ranges): the form for activation checkpoints.  round()
+ * is to nearest, halves to even, of the exact quotient.  A column of zeros has scale 0; one that holds a NaN, an infinity or a
+ * value beyond 127 * 2^121 gets scale NaN and q = 0. */
+int sgemm_i8_quantize(sgemm_handle *h, const void *dX, int x_type, int8_t *dQ, float *dScale, uint32_t k, uint32_t n,
+                      uint32_t ldx, uint32_t ldq, int pow2, void *stream);
+
+/* The way back: out[:, j] = scale[j] * q[:, j], rounded to out_type. */
+int sgemm_i8_restore(sgemm_handle *h, const int8_t *dQ, const float *dScale, void *dOut, int out_type, uint32_t k, uint32_t n,
+                     uint32_t ldq, uint32_t ldo, void *stream);
+
+/* Root-mean-square norm with the residual's addition and an 8-bit result, per column of X (K x N in x_type, K > 0):
+ * h = x + residual and p = h * gamma in FP32; scale = P / 127 * rsqrt(mean h^2 + eps) with P = max |p|; q = round(127 p / P).
+ * dResidual may be NULL (h = x).  dSum, unless NULL, receives h rounded to x_type and may be dResidual or dX itself (same
+ * leading dimension).  gamma, residual and sum have x_type.  Columns as in sgemm_i8_quantize when P is 0 or out of range. */
+int sgemm_i8_rmsnorm(sgemm_handle *h, const void *dX, const void *dResidual, const void *dGamma, int x_type, float eps,
+                     int8_t *dQ, float *dScale, void *dSum, uint32_t k, uint32_t n, uint32_t ldx, uint32_t ldr,
+                     uint32_t ldq, uint32_t lds, void *stream);
+
+/* Weight gradient of a linear layer from its input's 8-bit checkpoint:
+ *   D[i, j] = alpha * sum_t V(q[i, t], scale[t]) * G[j, t] + beta * C[i, j]
+ * for M features, N channels and T tokens: q M x T int8, G (the output's gradient) N x T in g_type (FP16 or BF16), C and D
+ * M x N in d_type.  V(q, s) is s * q rounded to g_type, what sgemm_i8_restore gives (s * q itself for the scales of
+ * pow2).  C may be NULL when beta == 0 and may be D itself (same leading dimension).  Sums are FP32 in a fixed order: results are
+ * the same bits every time.  T = 0 gives beta * C. */
+int sgemm_i8_wgrad(sgemm_handle *h, const int8_t *dQ, const float *dScale, const void *dG, int g_type, const void *dC, void *dD,
+                   int d_type, float alpha, float beta, uint32_t m, uint32_t n, uint32_t tokens,
+                   uint32_t ldq, uint32_t ldg, uint32_t ldc, uint32_t ldd, void *stream);
+
 /* Tile rasterisation of the loaded kernel: xy[2*z], xy[2*z+1] = (tile x, tile y) of launch unit z for an
  * nx x ny tile grid, computed on the device by the kernel's own mapping function (the workgroup remap of
  * generator/generator.py:1437-1464). */
