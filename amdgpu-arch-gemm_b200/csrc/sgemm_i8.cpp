@@ -188,6 +188,13 @@ uint32_t i8_function_smem(int index, uint32_t main_smem) {
         if (f.index == index) return f.smem;
     return index == kWgrad ? (uint32_t)I8W_SMEM : index == kLinear ? main_smem : 0u;
 }
+int i8_wgrad_function() { return kWgrad; }
+uint32_t i8_wgrad_threads() { return I8W_THREADS; }
+const uint32_t *i8_layout(size_t *words) {
+    static const uint32_t layout[SGEMM_I8_LAYOUT_WORDS] = SGEMM_I8_LAYOUT;
+    *words = SGEMM_I8_LAYOUT_WORDS;
+    return layout;
+}
 int i8_function_registers(int index) { return index == kWgrad ? I8W_LAUNCH_REGS : 0; }
 
 }  // namespace sgemm_internal
@@ -346,11 +353,15 @@ SGEMM_API int sgemm_i8_wgrad(sgemm_handle *h, const int8_t *dQ, const float *dSc
     const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
     if (tiles > 0x3FFFFFFFull) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
     const uint32_t pairs = (uint32_t)std::max(1, v.sm_count / (int)kSmsPerPair), stages = ceil_div(tokens, I8W_BK);
-    // too few tiles for the device: cut the tokens into 2 or 4 parts that still run at the same time
+    // Too few tiles for the device: cut the tokens into as many parts (up to 4) as still run at the same time, with at least eight
+    // stages each.  (Clusters do not fill the device: 74 of 2 CTAs, but 33 of 4, 22 of 6 and 15 of 8 fit the
+    // 148 SMs with their uneven groups, and one cluster too many is a second wave: 16 tiles over 16384 tokens
+    // take 62 us in 2 parts and 71 in 4.)
     uint32_t parts = 1;
-    while (parts < 4 && tiles * parts * 2 <= pairs && stages >= parts * 8) parts *= 2;
-    if (v.split_k > 0) parts = v.split_k >= 4 ? 4u : v.split_k >= 2 ? 2u : 1u;
-    while (parts > 1 && stages < parts) parts /= 2;
+    for (uint32_t p = 2; p <= 4; ++p)
+        if (tiles <= v.wgrad_clusters[p] && stages >= p * 8) parts = p;
+    if (v.split_k > 0) parts = (uint32_t)std::min<int64_t>(v.split_k, 4);
+    parts = std::min(parts, stages);
     const uint32_t units = parts > 1 ? (uint32_t)tiles : (uint32_t)std::min<uint64_t>(tiles, pairs);
     const uint32_t grid = units * 2 * parts;
     I8TensorMap map_q, map_g;

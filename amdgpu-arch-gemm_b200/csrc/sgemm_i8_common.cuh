@@ -8,6 +8,8 @@
 
 #define I8_TIMEOUT_NS 2000000000ull
 
+extern "C" __device__ const uint32_t sgemm_i8_layout[SGEMM_I8_LAYOUT_WORDS] = SGEMM_I8_LAYOUT;   // read by sgemm_open
+
 struct alignas(64) I8TensorMap { uint64_t opaque[16]; };
 
 // ------------------------------------------------------------------------------- element types
@@ -65,6 +67,15 @@ __device__ __forceinline__ uint32_t i8_cluster_size() {
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
+// True in one lane of the (converged) warp, the same one every time.  The warps that issue MMAs and copies run their loops with all lanes
+// and elect one around the issuing instructions only: the compiler then knows the loop's values to be uniform and keeps
+// descriptors and addresses where those instructions take them from.  With a loop inside `if (lane == 0)` a stage of four MMAs took
+// its issuer 780 cycles, more than the 512 the tensor core needs for it.
+__device__ __forceinline__ bool i8_elect() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    return elected != 0u;
+}
 __device__ __forceinline__ void i8_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -75,9 +86,33 @@ __device__ __forceinline__ uint32_t i8_map_to_cta(uint32_t addr, uint32_t rank) 
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Shared memory by its 32-bit address.  (Through a pointer that was aligned by hand the compiler no longer knows the address
+// space and takes the generic instructions, whose latency is several times as long.  Volatile keeps their order among themselves
+// and to the barriers; loads issued before their values are needed stay under way together.)
+__device__ __forceinline__ uint4 i8_lds4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float i8_ldsf(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void i8_sts4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void i8_sts(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// Loads from a peer's shared memory.  (No "memory" clobber: several may be under way together; the cluster barriers before and
+// after them carry one.)
 __device__ __forceinline__ uint32_t i8_ld_cluster(uint32_t addr) {
     uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float4 i8_ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
 __device__ __forceinline__ void i8_mbar_init(uint32_t bar, uint32_t count) {
@@ -91,6 +126,13 @@ __device__ __forceinline__ void i8_mbar_arrive(uint32_t bar) {
 }
 __device__ __forceinline__ void i8_mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same with the instruction's default scope, for arrivals that publish nothing the waiting thread itself reads.  A release at cluster
+// scope makes the warp wait until all its earlier writes are visible to the whole cluster (900 cycles beside a busy tensor core).  What such an arrival
+// announces lies in this CTA's own shared memory and is read by the tensor core on the waiting thread's order: the
+// writes were handed to the asynchronous proxy by a proxy fence before (or were reads of TMEM, ordered by tcgen05 fences).
+__device__ __forceinline__ void i8_mbar_arrive_peer(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ uint32_t i8_mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -147,16 +189,15 @@ __device__ __forceinline__ void i8_mma_f16_pair(uint32_t d_tmem, uint64_t a_desc
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// Arrive on `bar` once every MMA issued so far by this thread has completed.  In a CTA pair the barrier exists in both
-// CTAs: the leader commits to its own copy and to the peer's.
-template <int GROUP> __device__ __forceinline__ void i8_commit(uint32_t bar, uint32_t peer_rank) {
-    if (GROUP == 2) {
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                     ::"r"(i8_map_to_cta(bar, peer_rank)) : "memory");
-    } else {
+// Arrive on `bar` once every MMA issued so far by this thread has completed.  In a CTA pair the barrier exists in both CTAs
+// at the same offset: the leader's one commit arrives on its own and on the peer's copy (`pair_mask`: the bits of the two CTAs'
+// ranks in the cluster).
+template <int GROUP> __device__ __forceinline__ void i8_commit(uint32_t bar, uint16_t pair_mask) {
+    if (GROUP == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(pair_mask) : "memory");
+    else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-    }
 }
 __device__ __forceinline__ void i8_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -177,10 +218,17 @@ __device__ __forceinline__ void i8_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) 
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void i8_tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void i8_tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // 64-bit shared-memory matrix descriptor: start address and the two byte offsets in 16-byte units, version 1, 128-byte
-// swizzle of 16-byte units.
+// swizzle of 16-byte units.  Moving the start address by `bytes` adds bytes / 16 to the descriptor (the field never carries: shared
+// memory ends below 256 KB), so the issuing thread keeps one descriptor per operand and adds constants: it issues an MMA every 128
+// cycles and has little time for address arithmetic.
 __device__ __forceinline__ uint64_t i8_smem_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo_bytes >> 4) << 16) | ((uint64_t)(sbo_bytes >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
@@ -217,6 +265,10 @@ __device__ __forceinline__ bool i8_wait_slow(const I8Wait &w, uint32_t bar, uint
 __device__ __forceinline__ bool i8_wait(const I8Wait &w, uint32_t bar, uint32_t parity, uint32_t tag, uint32_t tile, uint32_t kb) {
     if (i8_mbar_try_wait(bar, parity)) return true;
     return i8_wait_slow(w, bar, parity, tag, tile, kb);
+}
+// The same for a whole warp: true when the barrier completed for every lane.
+__device__ __forceinline__ bool i8_wait_warp(const I8Wait &w, uint32_t bar, uint32_t parity, uint32_t tag, uint32_t tile, uint32_t kb) {
+    return __all_sync(0xffffffffu, i8_wait(w, bar, parity, tag, tile, kb));
 }
 // After a wait gave up: copies and MMAs that may still be in flight get time to land before TMEM is released.
 __device__ __forceinline__ void i8_settle() {

@@ -46,13 +46,12 @@ struct I8LinearArgs {
     uint32_t tiles_m, tiles_n;
 };
 
-// Issue the four MMAs of one stage.
+// Issue the four MMAs of one stage: a step of 32 bytes of K inside the swizzled rows.
 template <int GROUP>
-__device__ __forceinline__ void i8_stage_mma(uint32_t d_tmem, uint32_t sw_addr, uint32_t sx_addr, uint32_t idesc, bool first) {
+__device__ __forceinline__ void i8_stage_mma(uint32_t d_tmem, uint64_t desc_w, uint64_t desc_x, uint32_t idesc, bool first) {
 #pragma unroll
     for (int kk = 0; kk < I8_BK / 32; ++kk)
-        i8_mma_s8<GROUP>(d_tmem, i8_smem_desc(sw_addr + kk * 32, 16, 1024), i8_smem_desc(sx_addr + kk * 32, 16, 1024), idesc,
-                         (first && kk == 0) ? 0u : 1u);
+        i8_mma_s8<GROUP>(d_tmem, desc_w + kk * 2, desc_x + kk * 2, idesc, (first && kk == 0) ? 0u : 1u);
 }
 
 // One TMEM lane's (channel's) accumulators of COLS tokens -> Y.  `sx` of token col0 + lane sits in lane `lane`.
@@ -140,42 +139,52 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
     sgemm_launch_dependents();
     sgemm_grid_dependency_wait();
 
-    if (warp == 0) {
-        if (lane == 0) {   // ---- TMA producer: both CTAs' loads report to the leader's "full" barrier
-            uint32_t stage = 0, phase = 0;
-            bool alive = true;
-            const uint32_t full_base = i8_map_to_cta(bar_full, 0u);
-            for (uint32_t tile = unit0; alive && tile < num_tiles; tile += unit_stride) {
-                uint32_t tx, ty;
-                sgemm_tile_raster(tile, a.tiles_m, a.tiles_n, OPT_WGM, tx, ty);
-                const int32_t m0 = (int32_t)(tx * 256 + rank * I8_BM), n0 = (int32_t)(ty * I8_BN + rank * I8_BN_CTA);
-                for (uint32_t kb = 0; kb < kbs; ++kb) {
-                    if (!i8_wait(waiter, bar_empty + 8 * stage, phase ^ 1u, 0x100u + stage, tile, kb)) { alive = false; break; }
-                    const uint32_t sw = smem_base + stage * I8_STAGE_BYTES, sx = sw + I8_W_BYTES;
+    if (warp == 0) {   // ---- TMA producer: both CTAs' loads report to the leader's "full" barrier
+        uint32_t stage = 0, phase = 0;
+        bool alive = true;
+        const uint32_t full_base = i8_map_to_cta(bar_full, 0u);
+        for (uint32_t tile = unit0; alive && tile < num_tiles; tile += unit_stride) {
+            uint32_t tx, ty;
+            sgemm_tile_raster(tile, a.tiles_m, a.tiles_n, OPT_WGM, tx, ty);
+            const int32_t m0 = (int32_t)(tx * 256 + rank * I8_BM), n0 = (int32_t)(ty * I8_BN + rank * I8_BN_CTA);
+            for (uint32_t kb = 0; kb < kbs; ++kb) {
+                if (!i8_wait_warp(waiter, bar_empty + 8 * stage, phase ^ 1u, 0x100u + stage, tile, kb)) { alive = false; break; }
+                const uint32_t sw = smem_base + stage * I8_STAGE_BYTES, sx = sw + I8_W_BYTES;
+                if (i8_elect()) {
                     if (rank == 0) i8_mbar_expect_tx(bar_full + 8 * stage, 2 * I8_STAGE_BYTES);
                     i8_tma_load_pair(sw, &map_w, full_base + 8 * stage, (int32_t)(kb * I8_BK), m0);
                     i8_tma_load_pair(sx, &map_x, full_base + 8 * stage, (int32_t)(kb * I8_BK), n0);
-                    if (++stage == I8_STAGES) { stage = 0; phase ^= 1u; }
                 }
+                if (++stage == I8_STAGES) { stage = 0; phase ^= 1u; }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {   // ---- MMA issuer
+        if (rank == 0) {   // ---- MMA issuer
             uint32_t stage = 0, phase = 0, handover = 0;
             bool alive = true;
+            const uint64_t desc_w0 = i8_smem_desc(smem_base, 16, 1024), desc_x0 = i8_smem_desc(smem_base + I8_W_BYTES, 16, 1024);
+            uint64_t desc_w = desc_w0, desc_x = desc_x0;
             for (uint32_t tile = unit0; alive && tile < num_tiles; tile += unit_stride, ++handover) {
                 const uint32_t buf = handover & 1u, acc_phase = (handover >> 1) & 1u;
-                if (!i8_wait(waiter, bar_tempty + 8 * buf, acc_phase ^ 1u, 0x200u + buf, tile, 0)) break;
+                if (!i8_wait_warp(waiter, bar_tempty + 8 * buf, acc_phase ^ 1u, 0x200u + buf, tile, 0)) break;
                 i8_fence_after();
                 for (uint32_t kb = 0; kb < kbs; ++kb) {
-                    if (!i8_wait(waiter, bar_full + 8 * stage, phase, 0x300u + stage, tile, kb)) { alive = false; break; }
+                    if (!i8_wait_warp(waiter, bar_full + 8 * stage, phase, 0x300u + stage, tile, kb)) { alive = false; break; }
                     i8_fence_after();
-                    const uint32_t sw = smem_base + stage * I8_STAGE_BYTES;
-                    i8_stage_mma<2>(tmem_base + buf * I8_BN, sw, sw + I8_W_BYTES, I8_IDESC(256, I8_BN), kb == 0);
-                    i8_commit<2>(bar_empty + 8 * stage, 1u);
-                    if (++stage == I8_STAGES) { stage = 0; phase ^= 1u; }
+                    if (i8_elect()) {
+                        i8_stage_mma<2>(tmem_base + buf * I8_BN, desc_w, desc_x, I8_IDESC(256, I8_BN), kb == 0);
+                        i8_commit<2>(bar_empty + 8 * stage, 3);
+                        if (kb + 1 == kbs) i8_commit<2>(bar_tfull + 8 * buf, 3);
+                    }
+                    desc_w += I8_STAGE_BYTES / 16;
+                    desc_x += I8_STAGE_BYTES / 16;
+                    if (++stage == I8_STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                        desc_w = desc_w0;
+                        desc_x = desc_x0;
+                    }
                 }
-                if (alive) i8_commit<2>(bar_tfull + 8 * buf, 1u);
             }
         }
     } else if (warp >= 4) {   // ---- epilogue: warps 4..7 the first half of the tile's tokens, 8..11 the second
@@ -192,7 +201,7 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
 #pragma unroll
             for (int c = 0; c < I8_EPI_COLS / 32; ++c) sx[c] = col0 + c * 32 + lane < a.n ? __ldg(a.sx + col0 + c * 32 + lane) : 0.0f;
             const uint32_t buf = handover & 1u, acc_phase = (handover >> 1) & 1u;
-            if (!__all_sync(0xffffffffu, i8_wait(waiter, bar_tfull + 8 * buf, acc_phase, 0x400u + buf, tile, 0))) break;
+            if (!i8_wait_warp(waiter, bar_tfull + 8 * buf, acc_phase, 0x400u + buf, tile, 0)) break;
             i8_fence_after();
 #pragma unroll
             for (int c = 0; c < I8_EPI_COLS / 32; ++c) {
@@ -202,7 +211,7 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
                 if (c + 1 == I8_EPI_COLS / 32) {   // the buffer is read: hand it back before the stores
                     i8_fence_before();
                     __syncwarp();
-                    if (lane == 0) i8_mbar_arrive_cluster(tempty_base + 8 * buf);
+                    if (lane == 0) i8_mbar_arrive_peer(tempty_base + 8 * buf);
                 }
                 i8_store_columns_any<32>(acc, a, channel, col0 + c * 32, sx[c], sw, bias);
             }
@@ -229,10 +238,10 @@ __device__ __forceinline__ void i8_linear_few(const I8LinearArgs &a, const I8Ten
     constexpr int CHUNK = TN < 32 ? TN : 32;
     static_assert(STAGES * STAGE_BYTES >= TN * I8_BM * 4, "the partial tile must fit the ring");
     static_assert(16 * STAGES + 16 <= 256, "barrier block size");
-    extern __shared__ uint8_t i8_smem_raw[];
-    const uint32_t smem_base = (i8_smem_u32(i8_smem_raw) + 1023u) & ~1023u;
+    extern __shared__ uint8_t i8_few_smem_raw[];
+    const uint32_t smem_base = (i8_smem_u32(i8_few_smem_raw) + 1023u) & ~1023u;
     const uint32_t bar_full = smem_base + STAGES * STAGE_BYTES, bar_empty = bar_full + 8 * STAGES, bar_done = bar_empty + 8 * STAGES;
-    uint8_t *generic_base = i8_smem_raw + (smem_base - i8_smem_u32(i8_smem_raw));
+    uint8_t *generic_base = i8_few_smem_raw + (smem_base - i8_smem_u32(i8_few_smem_raw));
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(generic_base + STAGES * STAGE_BYTES + 16 * STAGES + 8);
     volatile uint32_t *abort_flag = tmem_slot + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -263,30 +272,29 @@ __device__ __forceinline__ void i8_linear_few(const I8LinearArgs &a, const I8Ten
     sgemm_grid_dependency_wait();
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
-                if (!i8_wait(waiter, bar_empty + 8 * stage, phase ^ 1u, 0x110u + stage, tile, kb)) break;
-                const uint32_t sw = smem_base + stage * STAGE_BYTES, full = bar_full + 8 * stage;
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
+            if (!i8_wait_warp(waiter, bar_empty + 8 * stage, phase ^ 1u, 0x110u + stage, tile, kb)) break;
+            const uint32_t sw = smem_base + stage * STAGE_BYTES, full = bar_full + 8 * stage;
+            if (i8_elect()) {
                 i8_mbar_expect_tx(full, STAGE_BYTES);
                 i8_tma_load(sw, &map_w, full, (int32_t)(kb * I8_BK), (int32_t)(tx * I8_BM));
                 i8_tma_load(sw + I8_W_BYTES, &map_x, full, (int32_t)(kb * I8_BK), (int32_t)(ty * TN));
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            bool alive = true;
-            for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
-                if (!i8_wait(waiter, bar_full + 8 * stage, phase, 0x310u + stage, tile, kb)) { alive = false; break; }
-                i8_fence_after();
-                const uint32_t sw = smem_base + stage * STAGE_BYTES;
-                i8_stage_mma<1>(tmem_base, sw, sw + I8_W_BYTES, I8_IDESC(I8_BM, TN), kb == kb_begin);
-                i8_commit<1>(bar_empty + 8 * stage, 0u);
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t kb = kb_begin; kb < kb_end; ++kb) {
+            if (!i8_wait_warp(waiter, bar_full + 8 * stage, phase, 0x310u + stage, tile, kb)) break;
+            i8_fence_after();
+            const uint64_t desc_w = i8_smem_desc(smem_base, 16, 1024) + stage * (STAGE_BYTES / 16);
+            if (i8_elect()) {
+                i8_stage_mma<1>(tmem_base, desc_w, desc_w + I8_W_BYTES / 16, I8_IDESC(I8_BM, TN), kb == kb_begin);
+                i8_commit<1>(bar_empty + 8 * stage, 0);
+                if (kb + 1 == kb_end) i8_commit<1>(bar_done, 0);
             }
-            if (alive && kb_begin < kb_end) i8_commit<1>(bar_done, 0u);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
     }
     __syncwarp();
@@ -294,7 +302,7 @@ __device__ __forceinline__ void i8_linear_few(const I8LinearArgs &a, const I8Ten
     const float sw = channel < a.m ? __ldg(a.sw + channel) : 0.0f;
     const float bias = a.bias && channel < a.m ? __ldg(a.bias + channel) : 0.0f;
     const bool empty = kb_begin == kb_end;   // more parts than stages: this CTA's partial is zero
-    const bool done = empty || __all_sync(0xffffffffu, i8_wait(waiter, bar_done, 0u, 0x410u, tile, 0));
+    const bool done = empty || i8_wait_warp(waiter, bar_done, 0u, 0x410u, tile, 0);
     i8_fence_after();
     const uint32_t cols = min((uint32_t)TN, a.n - col_first);
     if (done) {
@@ -309,10 +317,10 @@ __device__ __forceinline__ void i8_linear_few(const I8LinearArgs &a, const I8Ten
                     const float sx = col_first + c * CHUNK + lane < a.n && lane < CHUNK ? __ldg(a.sx + col_first + c * CHUNK + lane) : 0.0f;
                     i8_store_columns_any<CHUNK>(acc, a, channel, col_first + c * CHUNK, sx, sw, bias);
                 } else {
-                    uint32_t *part = reinterpret_cast<uint32_t *>(generic_base) + c * CHUNK * I8_BM + threadIdx.x;
+                    const uint32_t part = smem_base + (c * CHUNK * I8_BM + threadIdx.x) * 4;
 #pragma unroll
                     for (int j = 0; j < CHUNK; ++j)
-                        if (c * CHUNK + j < cols) part[j * I8_BM] = empty ? 0u : acc[j];
+                        if (c * CHUNK + j < cols) i8_sts(part + j * (I8_BM * 4), empty ? 0u : acc[j]);
                 }
             }
         }
@@ -321,12 +329,26 @@ __device__ __forceinline__ void i8_linear_few(const I8LinearArgs &a, const I8Ten
         __syncwarp();
         i8_cluster_sync();
         if (done) {
-            for (uint32_t j = rank; j < cols; j += parts) {
-                int32_t sum = 0;
-                for (uint32_t p = 0; p < parts; ++p)
-                    sum += (int32_t)i8_ld_cluster(i8_map_to_cta(smem_base + (j * I8_BM + threadIdx.x) * 4, p));
-                const float v = fmaf((float)sum * __ldg(a.sx + col_first + j), sw, bias);
-                if (channel < a.m) i8_store(a.y, channel + (uint64_t)(col_first + j) * a.ldy, a.y_type, v);
+            // all parts of four tokens are under way together: a load from a peer is a long trip
+            for (uint32_t j0 = rank; j0 < cols; j0 += 4 * parts) {
+                int32_t v[4][8];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int p = 0; p < 8; ++p)
+                        v[u][p] = p < parts && j0 + u * parts < cols
+                                      ? (int32_t)i8_ld_cluster(i8_map_to_cta(smem_base + ((j0 + u * parts) * I8_BM + threadIdx.x) * 4, p)) : 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t j = j0 + u * parts;
+                    if (j < cols) {
+                        int32_t sum = 0;
+#pragma unroll
+                        for (int p = 0; p < 8; ++p) sum += v[u][p];
+                        const float y = fmaf((float)sum * __ldg(a.sx + col_first + j), sw, bias);
+                        if (channel < a.m) i8_store(a.y, channel + (uint64_t)(col_first + j) * a.ldy, a.y_type, y);
+                    }
+                }
             }
         }
         __syncwarp();

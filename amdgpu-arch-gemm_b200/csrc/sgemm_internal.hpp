@@ -64,6 +64,7 @@ struct I8View {
     int sm_count = 0;
     uint32_t tile_n = 0, main_threads = 0, main_smem = 0;   // the main linear kernel as generated
     int64_t force_variant = 0, split_k = 0;                 // options of sgemm_set_option
+    uint32_t wgrad_clusters[5] = {0, 0, 0, 0, 0};           // clusters of 2 * i CTAs of the weight gradient the device holds at a time
 };
 // False when the handle's cubin was not generated for INT8 operands.
 bool i8_view(sgemm_handle *h, I8View *view);
@@ -73,6 +74,10 @@ int i8_function_count();
 const char *i8_function_name(int index);
 uint32_t i8_function_smem(int index, uint32_t main_smem);
 int i8_function_registers(int index);
+int i8_wgrad_function();   // index of the weight gradient's kernel, and its block size
+uint32_t i8_wgrad_threads();
+// The words an INT8 cubin carries as `sgemm_i8_layout` when it was compiled from the sources of this library.
+const uint32_t *i8_layout(size_t *words);
 // Launch on the handle's context; cluster: CTAs per cluster (0: as compiled).
 int i8_launch(sgemm_handle *h, void *function, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, void *stream,
               void **params);

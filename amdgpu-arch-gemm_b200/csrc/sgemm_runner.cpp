@@ -30,7 +30,7 @@ namespace {
 #define DRIVER_FUNCTIONS(X)                                                                              \
     X(cuInit) X(cuDeviceGet) X(cuDeviceGetCount) X(cuDeviceGetAttribute) X(cuDevicePrimaryCtxRetain)     \
     X(cuDevicePrimaryCtxRelease) X(cuCtxPushCurrent) X(cuCtxPopCurrent) X(cuModuleLoad) X(cuModuleUnload) \
-    X(cuModuleGetFunction) X(cuFuncSetAttribute) X(cuFuncGetAttribute) X(cuLaunchKernel) X(cuLaunchKernelEx) X(cuTensorMapEncodeTiled) \
+    X(cuModuleGetFunction) X(cuModuleGetGlobal) X(cuOccupancyMaxActiveClusters) X(cuFuncSetAttribute) X(cuFuncGetAttribute) X(cuLaunchKernel) X(cuLaunchKernelEx) X(cuTensorMapEncodeTiled) \
     X(cuMemAlloc) X(cuMemFree) X(cuMemcpyHtoDAsync) X(cuMemcpyDtoHAsync) X(cuMemcpyHtoD) X(cuMemcpyDtoH) \
     X(cuMemsetD8) X(cuStreamSynchronize) X(cuCtxSynchronize) X(cuEventCreate)        \
     X(cuEventRecord) X(cuEventSynchronize) X(cuEventElapsedTime) X(cuEventDestroy) X(cuGetErrorString)   \
@@ -117,6 +117,7 @@ struct sgemm_handle {
     CUmodule module = nullptr;
     uint32_t elem_bytes = 4;    // size of an element of A and B: 4 (FP32), 2 (FP16 / BF16) or 1 (INT8), the latter two tensor variant only
     void *i8_functions[sgemm_internal::kI8Functions] = {};   // INT8 cubins: the kernels of the 8-bit entry points
+    uint32_t i8_wgrad_clusters[5] = {};                      // ... and how many clusters of 2 * i CTAs of the weight gradient run at a time
     CUfunction fn_pack16 = nullptr, fn_repitch = nullptr, fn_narrow16 = nullptr;
     CUfunction fn_main = nullptr, fn_simt = nullptr, fn_split_lo = nullptr, fn_pack_a = nullptr,
                fn_reduce = nullptr, fn_fill = nullptr, fn_tile_map = nullptr, fn_wait_selftest = nullptr;
@@ -981,6 +982,15 @@ SGEMM_API int sgemm_open(const char *cubin_path, const char *toml_path, int devi
         }
     }
     if (h->elem_bytes == 1) {   // the kernels of the 8-bit entry points
+        size_t words = 0, bytes = 0;
+        const uint32_t *layout = sgemm_internal::i8_layout(&words);
+        std::vector<uint32_t> found(words);
+        CUdeviceptr at = 0;
+        if ((r = d.cuModuleGetGlobal_(&at, &bytes, h->module, "sgemm_i8_layout")) != CUDA_SUCCESS || bytes != words * 4 ||
+            (r = d.cuMemcpyDtoH_(found.data(), at, bytes)) != CUDA_SUCCESS || std::memcmp(found.data(), layout, bytes) != 0) {
+            fail(h, SGEMM_ERR_MODULE, "'%s' was compiled from other sources than this library: rebuild both", cubin_path);
+            return bail(SGEMM_ERR_MODULE);
+        }
         for (int i = 0; i < sgemm_internal::i8_function_count(); ++i) {
             const char *name = sgemm_internal::i8_function_name(i);
             CUfunction fn = nullptr;
@@ -999,6 +1009,24 @@ SGEMM_API int sgemm_open(const char *cubin_path, const char *toml_path, int devi
                 return bail(SGEMM_ERR_MODULE);
             }
             h->i8_functions[i] = reinterpret_cast<void *>(fn);
+        }
+        const int wgrad = sgemm_internal::i8_wgrad_function();
+        for (uint32_t pairs = 1; pairs <= 4; ++pairs) {
+            CUlaunchAttribute cluster;
+            cluster.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+            cluster.value.clusterDim.x = 2 * pairs;
+            cluster.value.clusterDim.y = cluster.value.clusterDim.z = 1;
+            CUlaunchConfig lc;
+            std::memset(&lc, 0, sizeof lc);
+            lc.gridDimX = 2 * pairs * (uint32_t)h->sm_count;
+            lc.gridDimY = lc.gridDimZ = lc.blockDimY = lc.blockDimZ = 1;
+            lc.blockDimX = sgemm_internal::i8_wgrad_threads();
+            lc.sharedMemBytes = sgemm_internal::i8_function_smem(wgrad, 0);
+            lc.attrs = &cluster;
+            lc.numAttrs = 1;
+            int fit = 0;
+            if (d.cuOccupancyMaxActiveClusters_(&fit, reinterpret_cast<CUfunction>(h->i8_functions[wgrad]), &lc) != CUDA_SUCCESS) fit = 0;
+            h->i8_wgrad_clusters[pairs] = (uint32_t)std::max(fit, 0);
         }
     }
     if ((r = d.cuMemAlloc_(&h->status, kStatusAlloc * 4)) != CUDA_SUCCESS ||
@@ -1499,6 +1527,7 @@ bool i8_view(sgemm_handle *h, I8View *view) {
     view->main_smem = (uint32_t)h->cfg.dynamic_smem_bytes;
     view->force_variant = h->force_variant;
     view->split_k = h->split_k_opt;
+    for (int i = 0; i < 5; ++i) view->wgrad_clusters[i] = h->i8_wgrad_clusters[i];
     return true;
 }
 

@@ -151,18 +151,27 @@ def _ptr(x) -> int:
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
-_TYPE_CODES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_TYPE_CODES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3}
+_type_codes: dict = {}   # dtype object -> code, filled as dtypes are met
+
+
+def _dtype_code(dtype) -> int:
+    """Element type as the C ABI and the generator number it (0 FP32, 1 FP16, 2 BF16, 3 INT8), -1 for any other."""
+    code = _type_codes.get(dtype)
+    if code is None:
+        code = _type_codes[dtype] = _TYPE_CODES.get(str(dtype).replace("torch.", ""), -1)
+    return code
 
 
 def _type_code(x, given: Optional[int]) -> int:
-    """Element type of a matrix as the C ABI numbers it (0 FP32, 1 FP16, 2 BF16): the one given, else the tensor's or
-    array's own."""
+    """Element type of a matrix: the one given, else the tensor's or array's own (FP32, FP16 or BF16)."""
     if given is not None:
         return int(given)
-    name = str(getattr(x, "dtype", "")).replace("torch.", "")
-    if name not in _TYPE_CODES:
-        raise TypeError(f"element type {name or type(x).__name__!r}: pass a FP32, FP16 or BF16 tensor, or the type with an address")
-    return _TYPE_CODES[name]
+    code = _dtype_code(getattr(x, "dtype", None))
+    if not 0 <= code <= 2:
+        raise TypeError(f"element type of {type(x).__name__} {getattr(x, 'dtype', '')}: pass a FP32, FP16 or BF16 tensor, or the "
+                        f"type with an address")
+    return code
 
 
 class SgemmRunner:
@@ -234,16 +243,16 @@ class SgemmRunner:
                                                    lda, ldb, ldc, ldd), "sgemm_run_host_sharded")
 
     # ------------------------------------------------- 8-bit operands (cubins generated for INT8)
-    def _addr(self, x, name: str, dtype: Optional[str] = None) -> int:
+    def _addr(self, x, name: str, code: int = -1) -> int:
         """Address of an operand of an 8-bit call; a tensor must lie on the handle's GPU, have the element type the
-        call takes, and hold the elements of a row one after the other."""
-        if x is None or isinstance(x, int) or not hasattr(x, "data_ptr"):
+        call takes (`code`, -1: any), and hold the elements of a row one after the other."""
+        if not hasattr(x, "data_ptr"):
             return _ptr(x)
-        if not x.is_cuda or x.get_device() != self.device:
+        if x.get_device() != self.device:
             raise ValueError(f"{name} lies on {x.device}, the handle on GPU {self.device}")
-        if dtype is not None and str(x.dtype) != "torch." + dtype:
-            raise TypeError(f"{name} is {x.dtype}, the call takes {dtype}")
-        if x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
+        if code >= 0 and _dtype_code(x.dtype) != code:
+            raise TypeError(f"{name} is {x.dtype}, the call takes {[k for k, v in _TYPE_CODES.items() if v == code][0]}")
+        if not x.is_contiguous() and x.shape[-1] > 1 and x.stride(-1) != 1:
             raise ValueError(f"{name}: the elements of a row must be contiguous")
         return x.data_ptr()
 
@@ -252,21 +261,21 @@ class SgemmRunner:
         features; int8 W and X column-major K x M and K x N (a channel's weights, a token's features contiguous), Y
         column-major M x N in FP32, FP16 or BF16, scales and bias FP32."""
         self._check(self._L.sgemm_i8_linear(
-            self._h, self._addr(w, "w", "int8"), self._addr(w_scale, "w_scale", "float32"), self._addr(x, "x", "int8"),
-            self._addr(x_scale, "x_scale", "float32"), self._addr(bias, "bias", "float32"), self._addr(y, "y"),
+            self._h, self._addr(w, "w", 3), self._addr(w_scale, "w_scale", 0), self._addr(x, "x", 3),
+            self._addr(x_scale, "x_scale", 0), self._addr(bias, "bias", 0), self._addr(y, "y"),
             _type_code(y, y_type), m, n, k, ldw or max(k, 1), ldx or max(k, 1), ldy or max(m, 1), stream), "sgemm_i8_linear")
 
     def i8_quantize(self, x, q, scale, k, n, pow2=False, ldx=0, ldq=0, x_type=None, stream=0):
         """8-bit columns of the K x N matrix X with one scale each (a token's features or a channel's weights per column):
         scale max|x|/127, or with ``pow2`` the least power of two that holds the column (activation checkpoints)."""
         self._check(self._L.sgemm_i8_quantize(
-            self._h, self._addr(x, "x"), _type_code(x, x_type), self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"),
+            self._h, self._addr(x, "x"), _type_code(x, x_type), self._addr(q, "q", 3), self._addr(scale, "scale", 0),
             k, n, ldx or max(k, 1), ldq or max(k, 1), 1 if pow2 else 0, stream), "sgemm_i8_quantize")
 
     def i8_restore(self, q, scale, out, k, n, ldq=0, ldo=0, out_type=None, stream=0):
         """The values ``scale[j] * q[:, j]``, rounded to the output's type."""
         self._check(self._L.sgemm_i8_restore(
-            self._h, self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"), self._addr(out, "out"),
+            self._h, self._addr(q, "q", 3), self._addr(scale, "scale", 0), self._addr(out, "out"),
             _type_code(out, out_type), k, n, ldq or max(k, 1), ldo or max(k, 1), stream), "sgemm_i8_restore")
 
     def i8_rmsnorm(self, x, gamma, q, scale, k, n, residual=None, sum_out=None, eps=1e-6, ldx=0, ldr=0, ldq=0, lds=0,
@@ -274,21 +283,19 @@ class SgemmRunner:
         """Root-mean-square norm of X (+ residual) times gamma, as 8-bit columns with one scale each; ``sum_out`` receives
         X + residual in X's type (it may be the residual or X itself)."""
         code = _type_code(x, x_type)
-        dtype = None if x_type is not None else str(getattr(x, "dtype", "")).replace("torch.", "")
         self._check(self._L.sgemm_i8_rmsnorm(
-            self._h, self._addr(x, "x"), self._addr(residual, "residual", dtype), self._addr(gamma, "gamma", dtype),
-            code, eps, self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"),
-            self._addr(sum_out, "sum_out", dtype), k, n, ldx or k, ldr or k, ldq or k, lds or k, stream), "sgemm_i8_rmsnorm")
+            self._h, self._addr(x, "x"), self._addr(residual, "residual", code), self._addr(gamma, "gamma", code),
+            code, eps, self._addr(q, "q", 3), self._addr(scale, "scale", 0),
+            self._addr(sum_out, "sum_out", code), k, n, ldx or k, ldr or k, ldq or k, lds or k, stream), "sgemm_i8_rmsnorm")
 
     def i8_wgrad(self, q, scale, dy, dw, m, n, tokens, c=None, alpha=1.0, beta=0.0, ldq=0, lddy=0, ldc=0, lddw=0,
                  dy_type=None, dw_type=None, stream=0):
         """Weight gradient from an 8-bit checkpoint: dW[i, j] = alpha * sum_t V(q[i, t], scale[t]) * dY[j, t] + beta * C[i, j] with
         ``m`` features, ``n`` channels; V is the value ``i8_restore`` gives in dY's type (FP16 or BF16); C and dW have one type."""
         code = _type_code(dw, dw_type)
-        dtype = None if dw_type is not None else str(getattr(dw, "dtype", "")).replace("torch.", "")
         self._check(self._L.sgemm_i8_wgrad(
-            self._h, self._addr(q, "q", "int8"), self._addr(scale, "scale", "float32"), self._addr(dy, "dy"), _type_code(dy, dy_type),
-            self._addr(c, "c", dtype), self._addr(dw, "dw"), code, alpha, beta, m, n, tokens,
+            self._h, self._addr(q, "q", 3), self._addr(scale, "scale", 0), self._addr(dy, "dy"), _type_code(dy, dy_type),
+            self._addr(c, "c", code), self._addr(dw, "dw"), code, alpha, beta, m, n, tokens,
             ldq or max(m, 1), lddy or max(n, 1), ldc or max(m, 1), lddw or max(m, 1), stream), "sgemm_i8_wgrad")
 
     # ------------------------------------------------------------------------------- multi-GPU
