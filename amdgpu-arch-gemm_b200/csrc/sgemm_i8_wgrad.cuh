@@ -140,18 +140,32 @@ __device__ __forceinline__ float2 i8w_unpair(uint64_t v) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
     return r;
 }
+// sum2 += beta * C, eight columns at a time (as many as there are registers for).  L2 is asked for all of them first: lane l of the warp
+// covers columns l, l + 32, ... of its 32 rows.
 template <uint32_t TYPE>
-__device__ __forceinline__ void i8w_load_sums(uint64_t (&sum2)[64], const I8WgradArgs &a, uint32_t row, uint32_t col0) {
+__device__ __forceinline__ void i8w_add_c(uint64_t (&sum2)[64], const I8WgradArgs &a, uint32_t row, uint32_t row_first, uint32_t col0) {
     using E = I8Elem<TYPE>;
-    const typename E::type *c = static_cast<const typename E::type *>(a.c) + row + (uint64_t)col0 * a.ldc;
-    const uint32_t cols = row < a.m && col0 < a.n ? min(128u, a.n - col0) : 0u;
+    using T = typename E::type;
+    const T *c = static_cast<const T *>(a.c) + (uint64_t)col0 * a.ldc;
+    const uint32_t cols = col0 < a.n ? min(128u, a.n - col0) : 0u;
+    if (row_first < a.m) {
+        const uint32_t row_last = min(row_first + 31u, a.m - 1u);
+        for (uint32_t col = threadIdx.x & 31u; col < cols; col += 32) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(c + row_first + (uint64_t)col * a.ldc));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(c + row_last + (uint64_t)col * a.ldc));
+        }
+    }
+    const uint32_t mine = row < a.m ? cols : 0u;
+    c += row;
 #pragma unroll
-    for (int j = 0; j < 64; ++j) {
-        float v[2] = {0.0f, 0.0f};
+    for (int block = 0; block < 16; ++block) {
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 2; ++e, c += a.ldc)
-            if (2 * j + e < cols) v[e] = a.beta * E::get(*c);
-        sum2[j] = i8w_pair(v[0], v[1]);
+        for (int e = 0; e < 8; ++e) v[e] = block * 8 + e < mine ? E::get(c[(uint64_t)e * a.ldc]) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum2[block * 4 + e] = i8w_pair(a.beta * v[2 * e], a.beta * v[2 * e + 1]);
+        c += (uint64_t)8 * a.ldc;
+        asm volatile("" : "+l"(c)::"memory");
     }
 }
 template <uint32_t TYPE>
@@ -364,16 +378,16 @@ i8_wgrad(const __grid_constant__ I8WgradArgs a, const __grid_constant__ I8Tensor
             uint32_t tx, ty;
             sgemm_tile_raster(tile, a.tiles_m, a.tiles_n, OPT_WGM, tx, ty);
             const uint32_t row = tx * 256 + rank * 128 + quarter * 32 + i8w_feature(lane), col0 = ty * 256 + cbase;
-            // The running sum starts as beta * C: its 128 loads a lane are all under way while the tile's first chain is multiplied
-            // (taken one by one beside the stores they cost 4096 x 4096 in FP32 another 210 us).  The first part's sum has it.
+            // The running sum starts as beta * C, fetched while the tile's first chain is multiplied (taken one by one beside the stores, C
+            // cost 4096 x 4096 in FP32 another 210 us).  The first part's sum has it.
             uint64_t sum2[64];
-            if (a.beta != 0.0f && part == 0) {
-                if (a.d_type == SGEMM_I8_FP32) i8w_load_sums<SGEMM_I8_FP32>(sum2, a, row, col0);
-                else if (a.d_type == SGEMM_I8_BF16) i8w_load_sums<SGEMM_I8_BF16>(sum2, a, row, col0);
-                else i8w_load_sums<SGEMM_I8_FP16>(sum2, a, row, col0);
-            } else {
 #pragma unroll
-                for (int j = 0; j < 64; ++j) sum2[j] = 0ull;
+            for (int j = 0; j < 64; ++j) sum2[j] = 0ull;
+            if (a.beta != 0.0f && part == 0) {
+                const uint32_t row_first = tx * 256 + rank * 128 + quarter * 32;
+                if (a.d_type == SGEMM_I8_FP32) i8w_add_c<SGEMM_I8_FP32>(sum2, a, row, row_first, col0);
+                else if (a.d_type == SGEMM_I8_BF16) i8w_add_c<SGEMM_I8_BF16>(sum2, a, row, row_first, col0);
+                else i8w_add_c<SGEMM_I8_FP16>(sum2, a, row, row_first, col0);
             }
             const uint64_t alpha2 = i8w_pair(a.alpha, a.alpha);
             for (uint32_t kb = kb_begin; kb < kb_end; kb += i8w_chain_span(kb - kb_begin), ++handover) {
