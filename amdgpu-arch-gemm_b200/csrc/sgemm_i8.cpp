@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <utility>
 
 #define SGEMM_API extern "C" __attribute__((visibility("default")))
 
@@ -22,9 +23,9 @@ constexpr uint32_t kSmsPerPair = 2;
 // index of a kernel in the handle's table; the row kernels follow as [operation][type][form]
 enum : int {
     kFew16 = 0, kFew32, kFew64, kFew128, kWgrad, kWgradSimt, kLinear, kLinearSimt,
-    kQuantize,                                   // + 4 * type + form (vectors per thread 1, 2, 4; single elements)
-    kNorm = kQuantize + 12,
-    kRestore = kNorm + 12,                       // + 2 * type + (0 vectors, 1 single elements)
+    kQuantize,                                   // + 5 * type + form (8, 16, 32 elements per thread in aligned vectors; shifted vectors; single elements)
+    kNorm = kQuantize + 15,
+    kRestore = kNorm + 15,                       // + 2 * type + (0 aligned vectors, 1 shifted ones)
     kCount = kRestore + 6
 };
 static_assert(kCount <= kI8Functions, "the handle's table holds every kernel");
@@ -32,13 +33,13 @@ static_assert(kCount <= kI8Functions, "the handle's table holds every kernel");
 const char *const kNames[kCount] = {
     "i8_linear_few_16", "i8_linear_few_32", "i8_linear_few_64", "i8_linear_few_128", "i8_wgrad", "i8_wgrad_simt",
     "generated_gemm", "generated_gemm_simt",
-    "i8_quantize_fp32_v1", "i8_quantize_fp32_v2", "i8_quantize_fp32_v4", "i8_quantize_fp32_s4",
-    "i8_quantize_fp16_v1", "i8_quantize_fp16_v2", "i8_quantize_fp16_v4", "i8_quantize_fp16_s4",
-    "i8_quantize_bf16_v1", "i8_quantize_bf16_v2", "i8_quantize_bf16_v4", "i8_quantize_bf16_s4",
-    "i8_rmsnorm_fp32_v1", "i8_rmsnorm_fp32_v2", "i8_rmsnorm_fp32_v4", "i8_rmsnorm_fp32_s4",
-    "i8_rmsnorm_fp16_v1", "i8_rmsnorm_fp16_v2", "i8_rmsnorm_fp16_v4", "i8_rmsnorm_fp16_s4",
-    "i8_rmsnorm_bf16_v1", "i8_rmsnorm_bf16_v2", "i8_rmsnorm_bf16_v4", "i8_rmsnorm_bf16_s4",
-    "i8_restore_fp32_v", "i8_restore_fp32_s", "i8_restore_fp16_v", "i8_restore_fp16_s", "i8_restore_bf16_v", "i8_restore_bf16_s",
+    "i8_quantize_fp32_v1", "i8_quantize_fp32_v2", "i8_quantize_fp32_v4", "i8_quantize_fp32_u4", "i8_quantize_fp32_s4",
+    "i8_quantize_fp16_v1", "i8_quantize_fp16_v2", "i8_quantize_fp16_v4", "i8_quantize_fp16_u4", "i8_quantize_fp16_s4",
+    "i8_quantize_bf16_v1", "i8_quantize_bf16_v2", "i8_quantize_bf16_v4", "i8_quantize_bf16_u4", "i8_quantize_bf16_s4",
+    "i8_rmsnorm_fp32_v1", "i8_rmsnorm_fp32_v2", "i8_rmsnorm_fp32_v4", "i8_rmsnorm_fp32_u4", "i8_rmsnorm_fp32_s4",
+    "i8_rmsnorm_fp16_v1", "i8_rmsnorm_fp16_v2", "i8_rmsnorm_fp16_v4", "i8_rmsnorm_fp16_u4", "i8_rmsnorm_fp16_s4",
+    "i8_rmsnorm_bf16_v1", "i8_rmsnorm_bf16_v2", "i8_rmsnorm_bf16_v4", "i8_rmsnorm_bf16_u4", "i8_rmsnorm_bf16_s4",
+    "i8_restore_fp32_v", "i8_restore_fp32_u", "i8_restore_fp16_v", "i8_restore_fp16_u", "i8_restore_bf16_v", "i8_restore_bf16_u",
 };
 
 struct FewKernel {
@@ -91,7 +92,7 @@ int begin(sgemm_handle *h, const char *op, I8View *v) {
     return SGEMM_OK;
 }
 
-constexpr uint32_t kLargest = 0xFFFFFF00u;   // sizes above this would wrap when rounded up to a tile
+constexpr uint32_t kLargest = 0x7FFFFF00u;   // sizes above this would leave 31 bits when rounded up to a tile
 
 // ---------------------------------------------------------------------------------------------- linear
 struct LinearPlan {
@@ -152,29 +153,47 @@ int plan_linear(sgemm_handle *h, const I8View &v, const void *w, const void *x, 
 }
 
 // ------------------------------------------------------------------------------------------ row kernels
-// Threads per row and vectors per thread: the fewest threads that hold the row in four vectors each, then, while all rows
-// together would leave SMs without a block, twice as many threads with half the vectors.
-void plan_rows(const I8View &v, uint32_t k, uint32_t rows, uint32_t per_vector, bool vec, uint32_t *tpr, int *form) {
-    const uint32_t vectors = std::max(1u, (k + per_vector - 1) / per_vector);
-    uint32_t nv = 4, threads = 32;
-    while (threads < I8_ROW_MAX_THREADS && (uint64_t)threads * nv < vectors) threads *= 2;
-    if (vec)
-        while (nv > 1 && threads < I8_ROW_MAX_THREADS && (uint64_t)threads * nv >= vectors &&
-               (uint64_t)rows * threads < (uint64_t)v.sm_count * 2048) {
+// How the rows lie: all in aligned vectors; all starting at the same offset into one (so that one thread's elements are one vector of
+// each); or anyhow.
+enum RowForm { kRowsAligned, kRowsShifted, kRowsAnyhow };
+
+// Threads per row and elements per thread.  With many rows 32 elements a thread (256 threads hold 8192; longer rows are read twice);
+// while all rows together leave SMs short of threads, twice the threads with half the elements, down to 8: a few rows are
+// a matter of latency.
+void plan_rows(const I8View &v, uint32_t k, uint32_t rows, RowForm form, uint32_t *tpr, int *kernel) {
+    uint32_t per = 32, threads = 32;
+    const uint32_t elements = form == kRowsShifted ? k + 7 : k;   // (a shifted row reaches into one vector more)
+    while (threads < 256 && threads * per < elements) threads *= 2;
+    if (form == kRowsAligned) {
+        while (per > 8 && threads * per >= k / 2 && (uint64_t)rows * threads < (uint64_t)v.sm_count * 1024) {
             threads *= 2;
-            nv /= 2;
+            per /= 2;
         }
-    while (nv > 1 && vec && (uint64_t)threads * (nv / 2) >= vectors) nv /= 2;
+        while (per > 8 && threads * (per / 2) >= k) per /= 2;
+    }
     *tpr = threads;
-    *form = !vec ? 3 : nv == 4 ? 2 : nv == 2 ? 1 : 0;
+    *kernel = form == kRowsAnyhow ? 4 : form == kRowsShifted ? 3 : per == 32 ? 2 : per == 16 ? 1 : 0;
 }
 
-int launch_rows(sgemm_handle *h, const I8View &v, int base, int type, bool vec, RowArgs &a, void *stream) {
-    int form = 0;
-    plan_rows(v, a.k, a.rows, 16 / type_bytes(type), vec, &a.tpr, &form);
+// rows of `type` and their int8 images: x and, where there are, the residual and the sum
+RowForm row_form(int type, const RowArgs &a) {
+    const uint32_t eb = type_bytes(type), per = 16 / eb;
+    bool is_aligned = aligned(a.q, per) && a.ldq % per == 0 && (!a.g || aligned(a.g, 16)), alike = true;
+    const std::pair<const void *, uint32_t> rows[3] = {{a.x, a.ldx}, {a.r, a.ldr}, {a.sum, a.lds}};
+    for (const auto &m : rows) {
+        if (!m.first) continue;
+        is_aligned = is_aligned && aligned(m.first, 16) && (uint64_t)m.second * eb % 16 == 0;
+        alike = alike && ((uintptr_t)m.first - (uintptr_t)a.x) % 16 == 0 && ((uint64_t)m.second - a.ldx) * eb % 16 == 0;
+    }
+    return is_aligned ? kRowsAligned : alike ? kRowsShifted : kRowsAnyhow;
+}
+
+int launch_rows(sgemm_handle *h, const I8View &v, int base, int type, RowArgs &a, void *stream) {
+    int kernel = 0;
+    plan_rows(v, a.k, a.rows, row_form(type, a), &a.tpr, &kernel);
     const uint32_t threads = std::max<uint32_t>(I8_ROW_THREADS, a.tpr), per_block = threads / a.tpr;
     void *params[] = {&a};
-    return i8_launch(h, v.functions[base + 4 * type + form], ceil_div(a.rows, per_block), threads, 0, 0, stream, params);
+    return i8_launch(h, v.functions[base + 5 * type + kernel], ceil_div(a.rows, per_block), threads, 0, 0, stream, params);
 }
 
 }  // namespace
@@ -260,11 +279,10 @@ SGEMM_API int sgemm_i8_quantize(sgemm_handle *h, const void *dX, int x_type, int
     if (n == 0) return SGEMM_OK;
     if (k > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
     if (!dScale || (k && (!dX || !dQ))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X, Q or the scales are NULL");
-    const uint32_t eb = type_bytes(x_type), per = 16 / eb;
+    const uint32_t eb = type_bytes(x_type);
     if (!aligned(dX, eb) || !aligned(dScale, 4)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X or the scales are not aligned to their element type");
-    const bool vec = aligned(dX, 16) && (uint64_t)ldx * eb % 16 == 0 && aligned(dQ, per) && ldq % per == 0;
     RowArgs a{dX, nullptr, nullptr, nullptr, dQ, dScale, k, n, ldx, 0, 0, ldq, 32, (uint32_t)pow2, 0.0f};
-    return launch_rows(h, v, kQuantize, x_type, vec, a, stream);
+    return launch_rows(h, v, kQuantize, x_type, a, stream);
 }
 
 SGEMM_API int sgemm_i8_restore(sgemm_handle *h, const int8_t *dQ, const float *dScale, void *dOut, int out_type, uint32_t k,
@@ -282,7 +300,7 @@ SGEMM_API int sgemm_i8_restore(sgemm_handle *h, const int8_t *dQ, const float *d
     const uint32_t eb = type_bytes(out_type);
     if (!aligned(dOut, eb) || !aligned(dScale, 4)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "the output or the scales are not aligned to their element type");
     const bool vec = aligned(dQ, 16) && ldq % 16 == 0 && aligned(dOut, 16) && (uint64_t)ldo * eb % 16 == 0;
-    const uint64_t units = (uint64_t)(vec ? ceil_div(k, 16) : k) * n;
+    const uint64_t units = (uint64_t)(vec ? ceil_div(k, 16) : ceil_div(k, 16 / eb) + 1) * n;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((units + 255) / 256, (uint64_t)v.sm_count * 32);
     void *params[] = {&dQ, &dScale, &dOut, &k, &n, &ldq, &ldo};
     return i8_launch(h, v.functions[kRestore + 2 * out_type + (vec ? 0 : 1)], blocks, 256, 0, 0, stream, params);
@@ -303,16 +321,13 @@ SGEMM_API int sgemm_i8_rmsnorm(sgemm_handle *h, const void *dX, const void *dRes
     if (n == 0) return SGEMM_OK;
     if (k > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
     if (!dX || !dGamma || !dQ || !dScale) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X, gamma, Q or the scales are NULL");
-    const uint32_t eb = type_bytes(x_type), per = 16 / eb;
+    const uint32_t eb = type_bytes(x_type);
     if (!aligned(dX, eb) || !aligned(dGamma, eb) || !aligned(dResidual, eb) || !aligned(dSum, eb) || !aligned(dScale, 4))
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a matrix is not aligned to its element type");
     if ((dSum == dX && dX && lds != ldx) || (dSum == dResidual && dSum && lds != ldr))
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "the sum may replace X or the residual only with the same leading dimension");
-    auto vector_ok = [&](const void *p, uint32_t ld) { return !p || (aligned(p, 16) && (uint64_t)ld * eb % 16 == 0); };
-    const bool vec = vector_ok(dX, ldx) && vector_ok(dResidual, ldr) && vector_ok(dSum, lds) && aligned(dGamma, 16) &&
-                     aligned(dQ, per) && ldq % per == 0;
     RowArgs a{dX, dResidual, dGamma, dSum, dQ, dScale, k, n, ldx, ldr, lds, ldq, 32, 0, eps};
-    return launch_rows(h, v, kNorm, x_type, vec, a, stream);
+    return launch_rows(h, v, kNorm, x_type, a, stream);
 }
 
 SGEMM_API int sgemm_i8_wgrad(sgemm_handle *h, const int8_t *dQ, const float *dScale, const void *dG, int g_type, const void *dC,

@@ -35,9 +35,8 @@
 #define I8W_LAUNCH_REGS 72    // what 896 threads leave per thread; the register hand-over below starts from it
 #define I8W_CHAIN 8           // stages accumulated inside the tensor core before the sum moves to FP32 registers
 
-// ---- row kernels: 16-byte vectors of the input one thread keeps in registers
+// ---- row kernels: threads of a block (more when one row takes more)
 #define I8_ROW_THREADS 256
-#define I8_ROW_MAX_THREADS 1024
 
 // What a launch has to agree on with the kernel's code: the cubin carries these words, and sgemm_open compares them with the library's
 // own, so that a cubin and a library compiled from different sources are refused instead of running with too little shared memory.
@@ -45,7 +44,7 @@
     {                                                                                                                          \
         I8_FEW_SMEM(16, I8_FEW_STAGES_16), I8_FEW_SMEM(32, I8_FEW_STAGES_32), I8_FEW_SMEM(64, I8_FEW_STAGES_64),               \
             I8_FEW_SMEM(128, I8_FEW_STAGES_128), I8W_SMEM, I8W_BK, I8W_THREADS, I8_BM, I8_BK, I8_FEW_THREADS, I8_SIMT_TILE,    \
-            I8_SIMT_THREADS, I8_ROW_MAX_THREADS, SGEMM_I8_ARGS_VERSION                                                         \
+            I8_SIMT_THREADS, I8_ROW_THREADS, SGEMM_I8_ARGS_VERSION                                                         \
     }
 #define SGEMM_I8_LAYOUT_WORDS 14
 #define SGEMM_I8_ARGS_VERSION 1   // raised with every change of an argument structure

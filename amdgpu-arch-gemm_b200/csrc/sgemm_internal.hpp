@@ -56,7 +56,7 @@ int launch_with_scratch(sgemm_handle *h, void *scratch, size_t scratch_bytes, co
 struct alignas(64) I8TensorMap {
     uint64_t opaque[16];
 };
-constexpr int kI8Functions = 48;
+constexpr int kI8Functions = 64;
 // What the planner needs to know about a handle of an INT8 cubin.
 struct I8View {
     void *const *functions = nullptr;   // kernels by index (sgemm_i8.cpp numbers and names them)

@@ -158,10 +158,10 @@ def test_power_of_two_checkpoint_round_trip(r, kind):
     assert np.all(127 * s >= peak) and np.all(127 * s / 2 < peak)
 
 
-def rmsnorm(r, x, g, kind, residual=None, eps=1e-6, ld=None, ldq=None, offset=0, want_sum=True, inplace=None):
+def rmsnorm(r, x, g, kind, residual=None, eps=1e-6, ld=None, ldq=None, offset=0, want_sum=True, inplace=None, roffset=None, goffset=0):
     rows, k = x.shape
-    src, gb = Buffer(rows, k, kind, ld, offset, x), Buffer(1, k, kind, values=g[None])
-    res = Buffer(rows, k, kind, ld, offset, residual) if residual is not None else None
+    src, gb = Buffer(rows, k, kind, ld, offset, x), Buffer(1, k, kind, offset=goffset, values=g[None])
+    res = Buffer(rows, k, kind, ld, offset if roffset is None else roffset, residual) if residual is not None else None
     total = {"x": src, "residual": res, None: Buffer(rows, k, kind, ld, offset) if want_sum else None}[inplace]
     q, s = Buffer(rows, k, "int8", ldq, offset), Buffer(1, rows, "fp32")
     r.i8_rmsnorm(src.address, gb.address, q.address, s.address, k, rows, residual=res.address if res else None,
@@ -187,7 +187,7 @@ def test_rmsnorm(r, kind, with_residual, k):
     rows = 3 if k > 20000 else 21
     x, g = activations(rng, rows, k, kind), activations(rng, 1, k, kind, 0.0)[0]
     res = activations(rng, rows, k, kind, 2.0) if with_residual else None
-    check_norm(rmsnorm(r, x, g, kind, res), x, g, kind, res, passes=1 + k // 16384)
+    check_norm(rmsnorm(r, x, g, kind, res), x, g, kind, res, passes=1 + k // 8192)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -197,7 +197,34 @@ def test_rmsnorm_sum_in_place_and_pitches(r, kind, inplace, rows, k, ld, ldq, of
     rng = np.random.default_rng(k)
     x, res = activations(rng, rows, k, kind), activations(rng, rows, k, kind)
     g = activations(rng, 1, k, kind, 0.0)[0]
-    check_norm(rmsnorm(r, x, g, kind, res, ld=ld, ldq=ldq, offset=offset, inplace=inplace), x, g, kind, res, passes=1 + k // 16384)
+    check_norm(rmsnorm(r, x, g, kind, res, ld=ld, ldq=ldq, offset=offset, inplace=inplace), x, g, kind, res, passes=1 + k // 8192)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("k,ld,ldq,offset,roffset,goffset", [(1000, 1001, 1000, 3, 3, 1), (1000, 1001, 1003, 3, 2, 0), (257, 257, 272, 0, 0, 5),
+                                                             (9000, 9001, 9008, 1, 1, 0), (5, 7, 6, 2, 2, 0), (40, 41, 41, 7, 0, 3)])
+def test_rmsnorm_rows_that_start_anywhere(r, kind, k, ld, ldq, offset, roffset, goffset):
+    """Vectors shifted against the rows (all matrices alike) and rows that share no alignment at all."""
+    rng = np.random.default_rng(k + ld)
+    x, res = activations(rng, 23, k, kind), activations(rng, 23, k, kind)
+    g = activations(rng, 1, k, kind, 0.0)[0]
+    got = rmsnorm(r, x, g, kind, res, ld=ld, ldq=ldq, offset=offset, roffset=roffset, goffset=goffset)
+    check_norm(got, x, g, kind, res, passes=1 + k // 8192)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shift", range(8))
+def test_quantize_and_restore_at_every_offset(r, kind, shift):
+    """Rows of every start and several lengths within their 16-byte vectors, q at another offset."""
+    for k in (1, 6, 17, 100, 1031):
+        x = activations(np.random.default_rng(k), 13, k, kind)
+        for pow2 in (False, True):
+            got = quantize(r, x, kind, pow2, k + shift, k + 3, shift, 5)
+            check_quantize(got, x, pow2)
+        qb, sb, out = Buffer(13, k, "int8", k + 3, shift, got[0]), Buffer(1, 13, "fp32", values=got[1][None]), Buffer(13, k, kind, k + shift, 1)
+        r.i8_restore(qb.address, sb.address, out.address, k, 13, ldq=qb.ld, ldo=out.ld, out_type=KINDS.index(kind))
+        torch.cuda.synchronize()
+        assert out.untouched() and np.array_equal(out.numpy(), model.restore(got[0], got[1], kind))
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -147,8 +147,8 @@ def test_linear_plans_cover_the_output(lib):
 
 
 def test_row_plans_hold_the_row(lib):
+    per, most = {"v1": 8, "v2": 16, "v4": 32, "u4": 32, "s4": 32}, {"v1": 1024, "v2": 512, "v4": 256, "u4": 256, "s4": 256}
     for x_type in (0, 1, 2):
-        per = 4 if x_type == 0 else 8
         for k in (1, 7, 64, 250, 1000, 4096, 8192, 16384, 100000):
             for n in (1, 5, 100, 8192):
                 for ldx in ((k + 15) // 16 * 16, (k + 15) // 16 * 16 + 1):
@@ -156,12 +156,13 @@ def test_row_plans_hold_the_row(lib):
                     assert quantize(lib, h, k=k, n=n, ldx=ldx, ldq=(k + 15) // 16 * 16, x_type=x_type) == 0
                     rec = last(lib)
                     name = lib.seam_name(rec.function).decode()
+                    form = name[-2:]
                     assert name.startswith("i8_quantize_" + ("fp32", "fp16", "bf16")[x_type])
-                    assert (name[-2] == "v") == (ldx % 16 == 0)
+                    assert (form[0] == "v") == (ldx % 16 == 0)
                     assert rec.tpr in (32, 64, 128, 256, 512, 1024) and rec.threads == max(256, rec.tpr)
+                    assert rec.tpr <= most[form]                       # the block the kernel was compiled for
                     assert rec.grid == -(-n // (rec.threads // rec.tpr))
-                    # one pass, or as many threads as a block has
-                    assert rec.tpr * int(name[-1]) * per >= k or rec.tpr == 1024
+                    assert rec.tpr * per[form] >= min(k + 7 * (form == "u4"), 8192)         # one pass, up to 8192 elements
 
 
 def test_wgrad_plans_cover_the_gradient(lib):
@@ -178,15 +179,17 @@ def test_wgrad_plans_cover_the_gradient(lib):
                 assert list(rec.dims) == [m, t, n, t] and list(rec.box) == [128, 64, 64, 64] and rec.smem <= 232448
 
 
-def test_vectors_need_aligned_rows(lib):
+def test_row_forms_follow_alignment(lib):
     h = lib.seam_handle(1, 0, 0)
     form = lambda: lib.seam_name(last(lib).function).decode()[-2:]   # noqa: E731
     assert rmsnorm(lib, h) == 0 and form()[0] == "v"
-    for kwargs in (dict(x=A + 2), dict(g=A + 8), dict(r=A + 4), dict(total=A + 2), dict(ldx=65), dict(r=A, ldr=66), dict(ldq=65), dict(q=A + 4)):
+    for kwargs in (dict(x=A + 2), dict(g=A + 8), dict(ldx=65), dict(ldq=65), dict(q=A + 4), dict(x=A + 2, r=A + 18, total=3 * A + 2, ldx=65, ldr=65, lds=73)):
+        assert rmsnorm(lib, h, **kwargs) == 0 and form() == "u4", kwargs      # every matrix at the same offset into a vector
+    for kwargs in (dict(r=A + 4), dict(total=A + 2), dict(r=A, ldr=66), dict(x=A + 2, r=A), dict(ldx=65, total=2 * A)):
         assert rmsnorm(lib, h, **kwargs) == 0 and form() == "s4", kwargs
     assert restore(lib, h) == 0 and form() == "_v"
     for kwargs in (dict(q=A + 8), dict(ldq=72), dict(out=A + 8), dict(ldo=65)):
-        assert restore(lib, h, **kwargs) == 0 and form() == "_s", kwargs
+        assert restore(lib, h, **kwargs) == 0 and form() == "_u", kwargs
 
 
 def test_register_hand_over_is_checked_for_the_kernel_that_does_it(lib):
