@@ -105,9 +105,9 @@ __device__ __forceinline__ void i8_sts4(uint32_t addr, uint32_t x, uint32_t y, u
 __device__ __forceinline__ void i8_sts(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 // Loads from a peer's shared memory.  (No "memory" clobber: several may be under way together; the cluster barriers before and
 // after them carry one.)
-__device__ __forceinline__ uint32_t i8_ld_cluster(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+__device__ __forceinline__ uint4 i8_ld_cluster4u(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
 }
 __device__ __forceinline__ float4 i8_ld_cluster4(uint32_t addr) {

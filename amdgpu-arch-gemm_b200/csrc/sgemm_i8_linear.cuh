@@ -329,24 +329,37 @@ __device__ __forceinline__ void i8_linear_few(const I8LinearArgs &a, const I8Ten
         __syncwarp();
         i8_cluster_sync();
         if (done) {
-            // all parts of four tokens are under way together: a load from a peer is a long trip
-            for (uint32_t j0 = rank; j0 < cols; j0 += 4 * parts) {
-                int32_t v[4][8];
+            // a warp takes a token, a lane four channels of it (16 bytes of each partial); all parts of two tokens are under way together:
+            // a load from a peer is a long trip
+            const uint32_t first = tx * I8_BM + lane * 4;
+            float sw4[4], bias4[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+            for (int e = 0; e < 4; ++e) {
+                sw4[e] = first + e < a.m ? __ldg(a.sw + first + e) : 0.0f;
+                bias4[e] = a.bias && first + e < a.m ? __ldg(a.bias + first + e) : 0.0f;
+            }
+            for (uint32_t j0 = rank + warp * parts; j0 < cols; j0 += 8 * parts) {
+                uint4 v[2][8];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int p = 0; p < 8; ++p)
-                        v[u][p] = p < parts && j0 + u * parts < cols
-                                      ? (int32_t)i8_ld_cluster(i8_map_to_cta(smem_base + ((j0 + u * parts) * I8_BM + threadIdx.x) * 4, p)) : 0;
+                        v[u][p] = p < parts && j0 + u * 4 * parts < cols
+                                      ? i8_ld_cluster4u(i8_map_to_cta(smem_base + (j0 + u * 4 * parts) * (I8_BM * 4) + lane * 16, p)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const uint32_t j = j0 + u * parts;
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t j = j0 + u * 4 * parts;
                     if (j < cols) {
-                        int32_t sum = 0;
+                        uint32_t sum[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-                        for (int p = 0; p < 8; ++p) sum += v[u][p];
-                        const float y = fmaf((float)sum * __ldg(a.sx + col_first + j), sw, bias);
-                        if (channel < a.m) i8_store(a.y, channel + (uint64_t)(col_first + j) * a.ldy, a.y_type, y);
+                        for (int p = 0; p < 8; ++p) {
+                            sum[0] += v[u][p].x; sum[1] += v[u][p].y; sum[2] += v[u][p].z; sum[3] += v[u][p].w;
+                        }
+                        const float sx = __ldg(a.sx + col_first + j);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (first + e < a.m)
+                                i8_store(a.y, first + e + (uint64_t)(col_first + j) * a.ldy, a.y_type, fmaf((float)(int32_t)sum[e] * sx, sw4[e], bias4[e]));
                     }
                 }
             }

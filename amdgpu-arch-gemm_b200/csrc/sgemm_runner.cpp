@@ -999,6 +999,8 @@ SGEMM_API int sgemm_open(const char *cubin_path, const char *toml_path, int devi
             int regs = 0;
             if ((r = d.cuModuleGetFunction_(&fn, h->module, name)) != CUDA_SUCCESS ||
                 (smem && (r = d.cuFuncSetAttribute_(fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)smem)) != CUDA_SUCCESS) ||
+                // two blocks of the few-token kernels fit an SM: all of its memory as shared memory
+                (smem && (r = d.cuFuncSetAttribute_(fn, CU_FUNC_ATTRIBUTE_PREFERRED_SHARED_MEMORY_CARVEOUT, 100)) != CUDA_SUCCESS) ||
                 (expect && (r = d.cuFuncGetAttribute_(&regs, CU_FUNC_ATTRIBUTE_NUM_REGS, fn)) != CUDA_SUCCESS)) {
                 fail(h, SGEMM_ERR_MODULE, "entry point '%s' unusable in '%s': %s", name, cubin_path, cu_text(r).c_str());
                 return bail(SGEMM_ERR_MODULE);
