@@ -10,14 +10,17 @@ CUDA driver / device is present, the calls raise ``SgemmError``.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import subprocess
+import sys
 from pathlib import Path
 from typing import Optional, Tuple
 
 PKG_DIR = Path(__file__).resolve().parent.parent
 LIB_PATH = PKG_DIR / "build" / "libsgemm_runner.so"
 RUNNER_PATH = PKG_DIR / "build" / "GeneratorRunner"
+NATIVE_PATH = PKG_DIR / "build" / "_sgemm_native.so"
 
 _f32p = ctypes.POINTER(ctypes.c_float)
 _u32 = ctypes.c_uint32
@@ -101,8 +104,8 @@ _lib: Optional[ctypes.CDLL] = None
 
 def build_library(force: bool = False) -> Path:
     """Run the Makefile beside this file (g++ and nvcc; needs the CUDA toolkit headers, not a GPU)."""
-    if force or not LIB_PATH.exists() or not RUNNER_PATH.exists():
-        env = dict(os.environ)
+    if force or not LIB_PATH.exists() or not RUNNER_PATH.exists() or not NATIVE_PATH.exists():
+        env = dict(os.environ, PYTHON=sys.executable)
         env.pop("CXX", None)
         subprocess.run(["make", "-C", str(Path(__file__).resolve().parent), "-s"] + (["-B"] if force else []),
                        check=True, env=env)
@@ -122,6 +125,24 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+_native_module = None
+
+
+def _native():
+    """The extension module behind the ``i8_*`` methods (csrc/sgemm_py.cpp)."""
+    global _native_module
+    if _native_module is None:
+        lib()
+        if not NATIVE_PATH.exists():
+            raise SgemmError(-5, "_sgemm_native", f"{NATIVE_PATH} is not built; run __graft_entry__.build() or make -C {PKG_DIR / 'runner'}")
+        spec = importlib.util.spec_from_file_location("_sgemm_native", NATIVE_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.setup(_type_codes, _type_code)
+        _native_module = module
+    return _native_module
 
 
 def parse_config(toml_path: str) -> SgemmConfig:
@@ -187,6 +208,7 @@ class SgemmRunner:
             self._h = None
             raise SgemmError(rc, "sgemm_open", self._L.sgemm_last_error(None).decode())
         self.device = device
+        self._native = None
 
     # ---------------------------------------------------------------------------------- plumbing
     def _check(self, rc: int, what: str):
@@ -256,47 +278,42 @@ class SgemmRunner:
             raise ValueError(f"{name}: the elements of a row must be contiguous")
         return x.data_ptr()
 
+    def _i8(self, name: str, *args):
+        if not self._h:
+            raise SgemmError(-1, "sgemm_" + name, "the handle is closed")
+        native = self._native
+        if native is None:
+            native = self._native = _native()
+        rc = getattr(native, name)(self, self._h.value, self.device, *args)
+        if rc:
+            self._check(rc, "sgemm_" + name)
+
     def i8_linear(self, w, w_scale, x, x_scale, y, m, n, k, bias=None, ldw=0, ldx=0, ldy=0, y_type=None, stream=0):
         """Y[i, j] = (sum_k W[k, i] X[k, j]) * x_scale[j] * w_scale[i] (+ bias[i]): ``m`` channels, ``n`` tokens, ``k``
         features; int8 W and X column-major K x M and K x N (a channel's weights, a token's features contiguous), Y
         column-major M x N in FP32, FP16 or BF16, scales and bias FP32."""
-        self._check(self._L.sgemm_i8_linear(
-            self._h, self._addr(w, "w", 3), self._addr(w_scale, "w_scale", 0), self._addr(x, "x", 3),
-            self._addr(x_scale, "x_scale", 0), self._addr(bias, "bias", 0), self._addr(y, "y"),
-            _type_code(y, y_type), m, n, k, ldw or max(k, 1), ldx or max(k, 1), ldy or max(m, 1), stream), "sgemm_i8_linear")
+        self._i8("i8_linear", w, w_scale, x, x_scale, y, m, n, k, bias, ldw, ldx, ldy, y_type, stream)
 
     def i8_quantize(self, x, q, scale, k, n, pow2=False, ldx=0, ldq=0, x_type=None, stream=0):
         """8-bit columns of the K x N matrix X with one scale each (a token's features or a channel's weights per column):
         scale max|x|/127, or with ``pow2`` the least power of two that holds the column (activation checkpoints)."""
-        self._check(self._L.sgemm_i8_quantize(
-            self._h, self._addr(x, "x"), _type_code(x, x_type), self._addr(q, "q", 3), self._addr(scale, "scale", 0),
-            k, n, ldx or max(k, 1), ldq or max(k, 1), 1 if pow2 else 0, stream), "sgemm_i8_quantize")
+        self._i8("i8_quantize", x, q, scale, k, n, pow2, ldx, ldq, x_type, stream)
 
     def i8_restore(self, q, scale, out, k, n, ldq=0, ldo=0, out_type=None, stream=0):
         """The values ``scale[j] * q[:, j]``, rounded to the output's type."""
-        self._check(self._L.sgemm_i8_restore(
-            self._h, self._addr(q, "q", 3), self._addr(scale, "scale", 0), self._addr(out, "out"),
-            _type_code(out, out_type), k, n, ldq or max(k, 1), ldo or max(k, 1), stream), "sgemm_i8_restore")
+        self._i8("i8_restore", q, scale, out, k, n, ldq, ldo, out_type, stream)
 
     def i8_rmsnorm(self, x, gamma, q, scale, k, n, residual=None, sum_out=None, eps=1e-6, ldx=0, ldr=0, ldq=0, lds=0,
                    x_type=None, stream=0):
         """Root-mean-square norm of X (+ residual) times gamma, as 8-bit columns with one scale each; ``sum_out`` receives
         X + residual in X's type (it may be the residual or X itself)."""
-        code = _type_code(x, x_type)
-        self._check(self._L.sgemm_i8_rmsnorm(
-            self._h, self._addr(x, "x"), self._addr(residual, "residual", code), self._addr(gamma, "gamma", code),
-            code, eps, self._addr(q, "q", 3), self._addr(scale, "scale", 0),
-            self._addr(sum_out, "sum_out", code), k, n, ldx or k, ldr or k, ldq or k, lds or k, stream), "sgemm_i8_rmsnorm")
+        self._i8("i8_rmsnorm", x, gamma, q, scale, k, n, residual, sum_out, eps, ldx, ldr, ldq, lds, x_type, stream)
 
     def i8_wgrad(self, q, scale, dy, dw, m, n, tokens, c=None, alpha=1.0, beta=0.0, ldq=0, lddy=0, ldc=0, lddw=0,
                  dy_type=None, dw_type=None, stream=0):
         """Weight gradient from an 8-bit checkpoint: dW[i, j] = alpha * sum_t V(q[i, t], scale[t]) * dY[j, t] + beta * C[i, j] with
         ``m`` features, ``n`` channels; V is the value ``i8_restore`` gives in dY's type (FP16 or BF16); C and dW have one type."""
-        code = _type_code(dw, dw_type)
-        self._check(self._L.sgemm_i8_wgrad(
-            self._h, self._addr(q, "q", 3), self._addr(scale, "scale", 0), self._addr(dy, "dy"), _type_code(dy, dy_type),
-            self._addr(c, "c", code), self._addr(dw, "dw"), code, alpha, beta, m, n, tokens,
-            ldq or max(m, 1), lddy or max(n, 1), ldc or max(m, 1), lddw or max(m, 1), stream), "sgemm_i8_wgrad")
+        self._i8("i8_wgrad", q, scale, dy, dw, m, n, tokens, c, alpha, beta, ldq, lddy, ldc, lddw, dy_type, dw_type, stream)
 
     # ------------------------------------------------------------------------------- multi-GPU
     def comm_init(self, comm_id: bytes, rank: int, world: int):
