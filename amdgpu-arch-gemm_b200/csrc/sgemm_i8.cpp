@@ -22,7 +22,7 @@ constexpr uint32_t kSmsPerPair = 2;
 
 // index of a kernel in the handle's table; the row kernels follow as [operation][type][form]
 enum : int {
-    kFew16 = 0, kFew32, kFew64, kFew128, kWgrad, kWgradSimt, kLinear, kLinearSimt,
+    kFew16 = 0, kFew32, kFew64, kFew128, kWgrad, kWgradSimt, kLinear, kHalf, kLinearSimt,
     kQuantize,                                   // + 5 * type + form (8, 16, 32 elements per thread in aligned vectors; shifted vectors; single elements)
     kNorm = kQuantize + 15,
     kRestore = kNorm + 15,                       // + 2 * type + (0 aligned vectors, 1 shifted ones)
@@ -32,7 +32,7 @@ static_assert(kCount <= kI8Functions, "the handle's table holds every kernel");
 
 const char *const kNames[kCount] = {
     "i8_linear_few_16", "i8_linear_few_32", "i8_linear_few_64", "i8_linear_few_128", "i8_wgrad", "i8_wgrad_simt",
-    "generated_gemm", "generated_gemm_simt",
+    "generated_gemm", "i8_linear_half", "generated_gemm_simt",
     "i8_quantize_fp32_v1", "i8_quantize_fp32_v2", "i8_quantize_fp32_v4", "i8_quantize_fp32_u4", "i8_quantize_fp32_s4",
     "i8_quantize_fp16_v1", "i8_quantize_fp16_v2", "i8_quantize_fp16_v4", "i8_quantize_fp16_u4", "i8_quantize_fp16_s4",
     "i8_quantize_bf16_v1", "i8_quantize_bf16_v2", "i8_quantize_bf16_v4", "i8_quantize_bf16_u4", "i8_quantize_bf16_s4",
@@ -101,53 +101,60 @@ struct LinearPlan {
     uint32_t parts = 1;
 };
 
-// Parts of K for the few-token kernel: the cut with the least work on the longest-running SM.  A CTA costs its stages plus a
-// fixed share (set-up, first loads, reduction: about four stages); `slots` of them run at a time.
-uint32_t cut_k(uint32_t tiles, uint32_t stages, uint32_t slots, uint64_t *cost) {
-    uint32_t best = 1;
-    uint64_t best_cost = ~0ull;
-    for (uint32_t parts = 1; parts <= 8 && parts <= std::max(1u, stages / 2); parts *= 2) {
-        const uint64_t waves = ((uint64_t)tiles * parts + slots - 1) / slots;
-        const uint64_t c = waves * (ceil_div(stages, parts) + 4);
-        if (c < best_cost) { best_cost = c; best = parts; }
-    }
-    if (cost) *cost = best_cost;
-    return best;
+// Estimated nanoseconds of a call on each kernel, fitted to calls back to back on a B200 (captured graphs, weights out of L2); the
+// estimates meet the measured times of 17 shapes between (1, 4096, 4096) and (2048, 4096, 4096) within 15 %.  What matters is where
+// they cross: (tokens, channels, features) = (509, 4096, 4096) takes 14.9 us on 256 x 256 tiles, 10.8 on 256 x 128
+// and 14.2 on 128 x 128; (1024, 4096, 4096) 15.8, 17.2 and 26.8; (64, 4096, 4096) 14.8, 10.0 and, cut in 4 parts, 9.2.
+//   pairs: set-up and the first loads, then so many waves of tiles with a stage every 320 ns (256 x 256) or 190 (256 x 128)
+uint64_t pair_ns(uint64_t tiles, uint32_t pairs, uint32_t stages, bool half) {
+    const uint64_t waves = (tiles + pairs - 1) / pairs;
+    return half ? 4400 + waves * stages * 190 : 5000 + waves * stages * 320;
+}
+//   few tokens: a stage's cost is the latency of its loads over the depth of the ring; a cut adds the cluster's barriers and the sum over
+//   the parts, and is limited by how many clusters the device holds (148 SMs in uneven groups); never below the weights' trip from memory
+uint64_t few_ns(const FewKernel &f, uint64_t tiles, uint32_t stages, uint32_t parts, uint32_t sms, uint64_t bytes) {
+    const uint32_t per_sm = f.tile_n <= 64 ? 2 : 1;
+    const uint64_t slots = per_sm * (parts == 1 ? sms : parts == 2 ? sms / 2 : parts == 4 ? sms * 33 / 148 : sms * 15 / 148);
+    const uint64_t waves = (tiles + std::max<uint64_t>(slots, 1) - 1) / std::max<uint64_t>(slots, 1);
+    const uint64_t stage = f.tile_n == 128 ? 345 : f.tile_n == 64 ? 317 : f.tile_n == 32 ? 270 : 236;
+    const uint64_t ns = 2000 + waves * ceil_div(stages, parts) * stage + (parts > 1 ? 1100 + 40ull * f.tile_n : 0);
+    return std::max<uint64_t>(ns, 3500 + bytes / 6000) + ns / 8;   // (where memory decides, the cut with more loads under way)
 }
 
 int plan_linear(sgemm_handle *h, const I8View &v, const void *w, const void *x, uint32_t m, uint32_t n, uint32_t k,
                 uint32_t ldw, uint32_t ldx, LinearPlan *p) {
     const bool tma = aligned(w, 16) && aligned(x, 16) && ldw % 16 == 0 && ldx % 16 == 0;
-    if (v.force_variant == 1 || v.force_variant == 3) {
-        if (!tma || k == 0)
-            return refuse(h, SGEMM_ERR_UNSUPPORTED, "sgemm_i8_linear",
-                          "a tensor kernel is forced but the operands need 16-byte aligned bases, leading dimensions that are multiples of 16 and K > 0");
-    }
+    if (v.force_variant != 0 && v.force_variant != 2 && (!tma || k == 0))
+        return refuse(h, SGEMM_ERR_UNSUPPORTED, "sgemm_i8_linear",
+                      "a tensor kernel is forced but the operands need 16-byte aligned bases, leading dimensions that are multiples of 16 and K > 0");
     if (v.force_variant == 2 || !tma || k == 0) {
         p->index = kLinearSimt;
         return SGEMM_OK;
     }
-    const uint32_t sms = (uint32_t)std::max(v.sm_count, 2), stages = ceil_div(k, I8_BK);
-    const uint32_t pairs_m = ceil_div(m, 256), pairs_n = ceil_div(n, v.tile_n);
-    // the few-token kernel whose tile holds all tokens, else the widest
+    p->index = v.force_variant == 4 ? kHalf : kLinear;
+    if (v.force_variant == 1 || v.force_variant == 4) return SGEMM_OK;
+    const uint32_t sms = (uint32_t)std::max(v.sm_count, 2), pairs = sms / kSmsPerPair, stages = ceil_div(k, I8_BK);
+    const uint64_t full = pair_ns((uint64_t)ceil_div(m, 256) * ceil_div(n, v.tile_n), pairs, stages, false);
+    const uint64_t half = pair_ns((uint64_t)ceil_div(m, 256) * ceil_div(n, I8_HALF_BN), pairs, stages, true);
+    uint64_t best = std::min(full, half);
+    if (half < full) p->index = kHalf;
+    // the few-token kernel whose tile holds all tokens (the widest takes more than one tile only when it is forced)
     const FewKernel *few = &kFew[3];
     for (const FewKernel &f : kFew)
         if (n <= f.tile_n) { few = &f; break; }
-    const uint64_t few_tiles = (uint64_t)ceil_div(m, I8_BM) * ceil_div(n, few->tile_n);
-    bool use_few = v.force_variant == 3;
-    uint32_t parts = 1;
-    if (v.force_variant != 1 && few_tiles * 8 < 0x7FFFFFFFull) {
-        uint64_t few_cost = 0;
-        parts = cut_k((uint32_t)few_tiles, stages, sms * (few->tile_n <= 64 ? 2 : 1), &few_cost);
-        // a pair's stage is 256 x 256 x 128 in 512 tensor cycles, a 128 x 128 one about 320 (bound by shared memory)
-        const uint64_t pair_waves = ((uint64_t)pairs_m * pairs_n + sms / kSmsPerPair - 1) / (sms / kSmsPerPair);
-        if (!use_few) use_few = n <= 128 || few_cost * 320 < pair_waves * (stages + 6) * 512;
-        if (v.split_k > 0) parts = v.split_k >= 8 ? 8u : v.split_k >= 4 ? 4u : v.split_k >= 2 ? 2u : 1u;
-    }
-    if (use_few) {
-        p->index = few->index;
-        p->few = few;
-        p->parts = parts;
+    const uint64_t tiles = (uint64_t)ceil_div(m, I8_BM) * ceil_div(n, few->tile_n);
+    if (v.force_variant == 3) best = ~0ull;
+    else if (n > few->tile_n) return SGEMM_OK;
+    for (uint32_t parts = 1; parts <= 8; parts *= 2) {
+        if (v.split_k > 0 && parts != (v.split_k >= 8 ? 8u : v.split_k >= 4 ? 4u : v.split_k >= 2 ? 2u : 1u)) continue;
+        if (v.split_k == 0 && parts > 1 && stages < 2 * parts) break;
+        const uint64_t ns = few_ns(*few, tiles, stages, parts, sms, (uint64_t)m * k);
+        if (ns < best) {
+            best = ns;
+            p->index = few->index;
+            p->few = few;
+            p->parts = parts;
+        }
     }
     return SGEMM_OK;
 }
@@ -205,7 +212,7 @@ const char *i8_function_name(int index) { return kNames[index]; }
 uint32_t i8_function_smem(int index, uint32_t main_smem) {
     for (const FewKernel &f : kFew)
         if (f.index == index) return f.smem;
-    return index == kWgrad ? (uint32_t)I8W_SMEM : index == kLinear ? main_smem : 0u;
+    return index == kWgrad ? (uint32_t)I8W_SMEM : index == kLinear ? main_smem : index == kHalf ? (uint32_t)I8_PAIR_SMEM(I8_HALF_BN, I8_HALF_STAGES) : 0u;
 }
 int i8_wgrad_function() { return kWgrad; }
 uint32_t i8_wgrad_threads() { return I8W_THREADS; }
@@ -238,8 +245,9 @@ SGEMM_API int sgemm_i8_linear(sgemm_handle *h, const int8_t *dW, const float *dW
     LinearPlan p;
     if ((rc = plan_linear(h, v, dW, dX, m, n, k, ldw, ldx, &p))) return rc;
     LinearArgs a{dW, dWscale, dX, dXscale, dBias, dY, v.status, m, n, k, ldw, ldx, ldy, (uint32_t)y_type, 0, 0};
-    const uint32_t tile_m = p.index == kLinear ? 256 : p.few ? I8_BM : I8_SIMT_TILE;
-    const uint32_t tile_n = p.index == kLinear ? v.tile_n : p.few ? p.few->tile_n : I8_SIMT_TILE;
+    const bool pair = p.index == kLinear || p.index == kHalf;
+    const uint32_t tile_m = pair ? 256 : p.few ? I8_BM : I8_SIMT_TILE;
+    const uint32_t tile_n = p.index == kLinear ? v.tile_n : p.index == kHalf ? I8_HALF_BN : p.few ? p.few->tile_n : I8_SIMT_TILE;
     a.tiles_m = ceil_div(m, tile_m);
     a.tiles_n = ceil_div(n, tile_n);
     const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
@@ -261,8 +269,8 @@ SGEMM_API int sgemm_i8_linear(sgemm_handle *h, const int8_t *dW, const float *dW
         return rc;
     }
     const uint32_t grid = kSmsPerPair * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)std::max(1, v.sm_count / (int)kSmsPerPair));
-    rc = i8_launch(h, v.functions[kLinear], grid, v.main_threads, v.main_smem, 0, stream, params);
-    i8_note(h, 1, 1, grid, tile_n);
+    rc = i8_launch(h, v.functions[p.index], grid, I8_PAIR_THREADS, i8_function_smem(p.index, v.main_smem), 0, stream, params);
+    i8_note(h, p.index == kHalf ? 4 : 1, 1, grid, tile_n);
     return rc;
 }
 
@@ -350,7 +358,7 @@ SGEMM_API int sgemm_i8_wgrad(sgemm_handle *h, const int8_t *dQ, const float *dSc
     if (!aligned(dG, 2) || !aligned(dScale, 4) || !aligned(dD, type_bytes(d_type)) || (beta != 0.0f && !aligned(dC, type_bytes(d_type))))
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a matrix is not aligned to its element type");
     const bool tma = aligned(dQ, 16) && ldq % 16 == 0 && aligned(dG, 16) && ldg % 8 == 0 && tokens > 0;
-    if ((v.force_variant == 1 || v.force_variant == 3) && !tma)
+    if (v.force_variant != 0 && v.force_variant != 2 && !tma)
         return refuse(h, SGEMM_ERR_UNSUPPORTED, op, "the tensor kernel is forced but the operands need 16-byte aligned bases, ldq a multiple of 16, ldg of 8, and a token");
     WgradArgs a{dQ, dScale, dG, dC, dD, v.status, m, n, tokens, ldq, ldg, ldc, ldd, (uint32_t)g_type, (uint32_t)d_type, alpha, beta, 0, 0};
     if (!tma || v.force_variant == 2) {

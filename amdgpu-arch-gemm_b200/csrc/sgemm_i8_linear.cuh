@@ -19,6 +19,7 @@
 //                      epilogue of a tile runs beside the main loop of the next one.  A pair reads each operand tile once
 //                      per 256 rows of the other, half of what two single CTAs would, which is what lets shared memory
 //                      feed the 8-bit rate.
+//   i8_linear_half     the same on 256 channels x 128 tokens, for problems whose 256 x 256 tiles leave half of the SMs idle.
 //   i8_linear_few_TN   one CTA on 128 channels x TN tokens and one part of K; the CTAs of a cluster hold the parts of one tile
 //                      and add their int32 partials through distributed shared memory.  For few tokens the layer is bound
 //                      by reading W once: small tiles and a cut K put every SM on it, without a workspace in global
@@ -88,25 +89,23 @@ __device__ __forceinline__ void i8_store_columns_any(const uint32_t (&acc)[COLS]
 }
 
 // ------------------------------------------------------------------------------- many tokens: CTA pairs
-#define I8_BN_CTA (I8_BN / 2)                       // tokens of a tile this CTA keeps in shared memory
 #define I8_W_BYTES (I8_BM * I8_BK)
-#define I8_X_BYTES (I8_BN_CTA * I8_BK)
-#define I8_STAGE_BYTES (I8_W_BYTES + I8_X_BYTES)
-#define I8_THREADS 384
-#define I8_EPI_COLS (I8_BN / 2)                     // columns one of the two epilogue warps of a lane quarter drains
-#define I8_TMEM_COLS (2 * I8_BN <= 128 ? 128 : 2 * I8_BN <= 256 ? 256 : 512)
-static_assert(I8_BN % 64 == 0 && I8_BN <= 256, "two accumulators in TMEM, whole 32-column chunks per epilogue warp");
-static_assert(I8_STAGES * I8_STAGE_BYTES + 1024 + 256 <= 232448, "shared memory budget of one CTA");
-static_assert(16 * I8_STAGES + 32 + 8 <= 256, "barrier block size");
 
-extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
-generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I8TensorMap map_w, const __grid_constant__ I8TensorMap map_x) {
+template <int BN, int STAGES>
+__device__ __forceinline__ void i8_linear_pair(const I8LinearArgs &a, const I8TensorMap &map_w, const I8TensorMap &map_x) {
+    constexpr uint32_t BN_CTA = BN / 2;              // tokens of a tile this CTA keeps in shared memory
+    constexpr uint32_t STAGE_BYTES = I8_W_BYTES + BN_CTA * I8_BK;
+    constexpr uint32_t EPI_COLS = BN / 2;            // columns one of the two epilogue warps of a lane quarter drains
+    constexpr uint32_t TMEM_COLS = 2 * BN <= 128 ? 128 : 2 * BN <= 256 ? 256 : 512;
+    static_assert(BN % 64 == 0 && BN <= 256, "two accumulators in TMEM, whole 32-column chunks per epilogue warp");
+    static_assert(I8_PAIR_SMEM(BN, STAGES) <= 232448, "shared memory budget of one CTA");
+    static_assert(16 * STAGES + 32 + 8 <= 256, "barrier block size");
     extern __shared__ uint8_t i8_smem_raw[];
     const uint32_t smem_base = (i8_smem_u32(i8_smem_raw) + 1023u) & ~1023u;
-    const uint32_t bar_base = smem_base + I8_STAGES * I8_STAGE_BYTES;
+    const uint32_t bar_base = smem_base + STAGES * STAGE_BYTES;
     // barrier block: full[S] | empty[S] | tmem_full[2] | tmem_empty[2] | tmem base (u32) | abort (u32)
-    const uint32_t bar_full = bar_base, bar_empty = bar_base + 8 * I8_STAGES;
-    const uint32_t bar_tfull = bar_base + 16 * I8_STAGES, bar_tempty = bar_tfull + 16;
+    const uint32_t bar_full = bar_base, bar_empty = bar_base + 8 * STAGES;
+    const uint32_t bar_tfull = bar_base + 16 * STAGES, bar_tempty = bar_tfull + 16;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(i8_smem_raw + (bar_tempty + 16 - i8_smem_u32(i8_smem_raw)));
     volatile uint32_t *abort_flag = tmem_slot + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -117,7 +116,7 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
     const uint32_t kbs = (a.k + I8_BK - 1) / I8_BK;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < I8_STAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             i8_mbar_init(bar_full + 8 * s, 1);
             i8_mbar_init(bar_empty + 8 * s, 1);
         }
@@ -131,7 +130,7 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
         i8_prefetch_map(&map_w);
         i8_prefetch_map(&map_x);
     }
-    if (warp == 1) i8_tmem_alloc<2>(i8_smem_u32(tmem_slot), I8_TMEM_COLS);
+    if (warp == 1) i8_tmem_alloc<2>(i8_smem_u32(tmem_slot), TMEM_COLS);
     i8_fence_before();
     i8_cluster_sync();   // the peer's barriers must be initialised before anything is signalled to them
     i8_fence_after();
@@ -146,16 +145,16 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
         for (uint32_t tile = unit0; alive && tile < num_tiles; tile += unit_stride) {
             uint32_t tx, ty;
             sgemm_tile_raster(tile, a.tiles_m, a.tiles_n, OPT_WGM, tx, ty);
-            const int32_t m0 = (int32_t)(tx * 256 + rank * I8_BM), n0 = (int32_t)(ty * I8_BN + rank * I8_BN_CTA);
+            const int32_t m0 = (int32_t)(tx * 256 + rank * I8_BM), n0 = (int32_t)(ty * BN + rank * BN_CTA);
             for (uint32_t kb = 0; kb < kbs; ++kb) {
                 if (!i8_wait_warp(waiter, bar_empty + 8 * stage, phase ^ 1u, 0x100u + stage, tile, kb)) { alive = false; break; }
-                const uint32_t sw = smem_base + stage * I8_STAGE_BYTES, sx = sw + I8_W_BYTES;
+                const uint32_t sw = smem_base + stage * STAGE_BYTES, sx = sw + I8_W_BYTES;
                 if (i8_elect()) {
-                    if (rank == 0) i8_mbar_expect_tx(bar_full + 8 * stage, 2 * I8_STAGE_BYTES);
+                    if (rank == 0) i8_mbar_expect_tx(bar_full + 8 * stage, 2 * STAGE_BYTES);
                     i8_tma_load_pair(sw, &map_w, full_base + 8 * stage, (int32_t)(kb * I8_BK), m0);
                     i8_tma_load_pair(sx, &map_x, full_base + 8 * stage, (int32_t)(kb * I8_BK), n0);
                 }
-                if (++stage == I8_STAGES) { stage = 0; phase ^= 1u; }
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
     } else if (warp == 1) {
@@ -172,13 +171,13 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
                     if (!i8_wait_warp(waiter, bar_full + 8 * stage, phase, 0x300u + stage, tile, kb)) { alive = false; break; }
                     i8_fence_after();
                     if (i8_elect()) {
-                        i8_stage_mma<2>(tmem_base + buf * I8_BN, desc_w, desc_x, I8_IDESC(256, I8_BN), kb == 0);
+                        i8_stage_mma<2>(tmem_base + buf * BN, desc_w, desc_x, I8_IDESC(256, BN), kb == 0);
                         i8_commit<2>(bar_empty + 8 * stage, 3);
                         if (kb + 1 == kbs) i8_commit<2>(bar_tfull + 8 * buf, 3);
                     }
-                    desc_w += I8_STAGE_BYTES / 16;
-                    desc_x += I8_STAGE_BYTES / 16;
-                    if (++stage == I8_STAGES) {
+                    desc_w += STAGE_BYTES / 16;
+                    desc_x += STAGE_BYTES / 16;
+                    if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                         desc_w = desc_w0;
@@ -188,27 +187,27 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
             }
         }
     } else if (warp >= 4) {   // ---- epilogue: warps 4..7 the first half of the tile's tokens, 8..11 the second
-        const uint32_t quarter = warp & 3u, cbase = ((warp - 4) >> 2) * I8_EPI_COLS;
+        const uint32_t quarter = warp & 3u, cbase = ((warp - 4) >> 2) * EPI_COLS;
         const uint32_t tempty_base = i8_map_to_cta(bar_tempty, 0u);
         uint32_t handover = 0;
         for (uint32_t tile = unit0; tile < num_tiles; tile += unit_stride, ++handover) {
             uint32_t tx, ty;
             sgemm_tile_raster(tile, a.tiles_m, a.tiles_n, OPT_WGM, tx, ty);
-            const uint32_t channel = tx * 256 + rank * I8_BM + quarter * 32 + lane, col0 = ty * I8_BN + cbase;
+            const uint32_t channel = tx * 256 + rank * I8_BM + quarter * 32 + lane, col0 = ty * BN + cbase;
             const float sw = channel < a.m ? __ldg(a.sw + channel) : 0.0f;
             const float bias = a.bias && channel < a.m ? __ldg(a.bias + channel) : 0.0f;
-            float sx[I8_EPI_COLS / 32];
+            float sx[EPI_COLS / 32];
 #pragma unroll
-            for (int c = 0; c < I8_EPI_COLS / 32; ++c) sx[c] = col0 + c * 32 + lane < a.n ? __ldg(a.sx + col0 + c * 32 + lane) : 0.0f;
+            for (int c = 0; c < EPI_COLS / 32; ++c) sx[c] = col0 + c * 32 + lane < a.n ? __ldg(a.sx + col0 + c * 32 + lane) : 0.0f;
             const uint32_t buf = handover & 1u, acc_phase = (handover >> 1) & 1u;
             if (!i8_wait_warp(waiter, bar_tfull + 8 * buf, acc_phase, 0x400u + buf, tile, 0)) break;
             i8_fence_after();
 #pragma unroll
-            for (int c = 0; c < I8_EPI_COLS / 32; ++c) {
+            for (int c = 0; c < EPI_COLS / 32; ++c) {
                 uint32_t acc[32];
-                i8_tmem_ld32(tmem_base + ((quarter * 32u) << 16) + buf * I8_BN + cbase + c * 32, acc);
+                i8_tmem_ld32(tmem_base + ((quarter * 32u) << 16) + buf * BN + cbase + c * 32, acc);
                 i8_tmem_ld_wait();
-                if (c + 1 == I8_EPI_COLS / 32) {   // the buffer is read: hand it back before the stores
+                if (c + 1 == EPI_COLS / 32) {   // the buffer is read: hand it back before the stores
                     i8_fence_before();
                     __syncwarp();
                     if (lane == 0) i8_mbar_arrive_peer(tempty_base + 8 * buf);
@@ -223,9 +222,16 @@ generated_gemm(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I
     if (warp == 1) {
         if (*abort_flag) i8_settle();
         i8_fence_after();
-        i8_tmem_dealloc<2>(tmem_base, I8_TMEM_COLS);
+        i8_tmem_dealloc<2>(tmem_base, TMEM_COLS);
     }
 }
+#define I8_PAIR_KERNEL(NAME, BN, STAGES)                                                                            \
+    extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_PAIR_THREADS, 1)                      \
+    NAME(const __grid_constant__ I8LinearArgs a, const __grid_constant__ I8TensorMap map_w, const __grid_constant__ I8TensorMap map_x) { \
+        i8_linear_pair<BN, STAGES>(a, map_w, map_x);                                                                \
+    }
+I8_PAIR_KERNEL(generated_gemm, I8_BN, I8_STAGES)
+I8_PAIR_KERNEL(i8_linear_half, I8_HALF_BN, I8_HALF_STAGES)
 
 // ---------------------------------------------------------------- few tokens: K cut over the CTAs of a cluster
 // Cluster of S = 1, 2, 4 or 8 CTAs per tile (a launch attribute).  CTA r takes the r-th of S even parts of K's stages.  With S > 1

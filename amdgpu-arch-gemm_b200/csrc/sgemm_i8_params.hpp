@@ -11,6 +11,11 @@
 // ---- linear: k per stage (one 128-byte swizzle span of int8), rows of W per CTA
 #define I8_BK 128
 #define I8_BM 128
+// CTA pairs: each CTA holds 128 rows of W and half of the tile's tokens
+#define I8_PAIR_THREADS 384
+#define I8_PAIR_SMEM(bn, stages) ((stages) * (I8_BM + (bn) / 2) * I8_BK + 1024 + 256)
+#define I8_HALF_BN 128
+#define I8_HALF_STAGES 8
 // few-token kernels: tile 128 channels x TN tokens, one tile and one K range per CTA, the CTAs of a cluster share a tile
 #define I8_FEW_THREADS 128
 #define I8_FEW_SMEM(tn, stages) ((stages) * (I8_BM + (tn)) * I8_BK + 1024 + 256)
@@ -44,9 +49,10 @@
     {                                                                                                                          \
         I8_FEW_SMEM(16, I8_FEW_STAGES_16), I8_FEW_SMEM(32, I8_FEW_STAGES_32), I8_FEW_SMEM(64, I8_FEW_STAGES_64),               \
             I8_FEW_SMEM(128, I8_FEW_STAGES_128), I8W_SMEM, I8W_BK, I8W_THREADS, I8_BM, I8_BK, I8_FEW_THREADS, I8_SIMT_TILE,    \
+            I8_PAIR_SMEM(I8_HALF_BN, I8_HALF_STAGES), I8_PAIR_THREADS,                                                         \
             I8_SIMT_THREADS, I8_ROW_THREADS, SGEMM_I8_ARGS_VERSION                                                         \
     }
-#define SGEMM_I8_LAYOUT_WORDS 14
+#define SGEMM_I8_LAYOUT_WORDS 16
 #define SGEMM_I8_ARGS_VERSION 1   // raised with every change of an argument structure
 
 #endif

@@ -62,7 +62,7 @@ struct I8View {
     void *const *functions = nullptr;   // kernels by index (sgemm_i8.cpp numbers and names them)
     uint32_t *status = nullptr;         // device status words
     int sm_count = 0;
-    uint32_t tile_n = 0, main_threads = 0, main_smem = 0;   // the main linear kernel as generated
+    uint32_t tile_n = 0, main_smem = 0;   // the main linear kernel as generated
     int64_t force_variant = 0, split_k = 0;                 // options of sgemm_set_option
     uint32_t wgrad_clusters[5] = {0, 0, 0, 0, 0};           // clusters of 2 * i CTAs of the weight gradient the device holds at a time
 };

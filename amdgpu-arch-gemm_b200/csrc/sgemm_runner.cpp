@@ -1321,7 +1321,7 @@ SGEMM_API int sgemm_wait_selftest(sgemm_handle *h, uint32_t timeout_ms, uint32_t
 SGEMM_API int sgemm_set_option(sgemm_handle *h, const char *key, int64_t value) {
     if (!h || !key) return SGEMM_ERR_INVALID_ARGUMENT;
     const std::string k(key);
-    if (k == "force_variant" && value >= 0 && value <= 3) h->force_variant = value;
+    if (k == "force_variant" && value >= 0 && value <= (h->elem_bytes == 1 ? 4 : 3)) h->force_variant = value;
     else if (k == "skinny_below_intensity" && value >= 0) h->skinny_below_intensity = value;
     else if (k == "skinny_below_flops" && value >= 0) h->skinny_below_flops = value;
     else if (k == "repitch" && (value == 0 || value == 1)) h->repitch = value != 0;
@@ -1525,7 +1525,6 @@ bool i8_view(sgemm_handle *h, I8View *view) {
     view->status = reinterpret_cast<uint32_t *>(h->status);
     view->sm_count = h->sm_count;
     view->tile_n = h->tile_n;
-    view->main_threads = (uint32_t)h->cfg.num_threads;
     view->main_smem = (uint32_t)h->cfg.dynamic_smem_bytes;
     view->force_variant = h->force_variant;
     view->split_k = h->split_k_opt;

@@ -276,7 +276,8 @@ int sgemm_narrow16(sgemm_handle *h, const float *dsrc, void *ddst, uint64_t coun
  * is served; 8-bit matrices whose base and leading dimension are multiples of 16 bytes (and G likewise) run on the
  * tensor cores, others on slower kernels.  Outputs must not overlap inputs except where a call says so; elements between
  * a column's K and its leading dimension are neither read nor written.  Options "force_variant" (0 auto, 1 tensor main
- * kernel, 2 fallback, 3 tensor few-token kernel) and "split_k" (parts of the sum, rounded down to 1, 2, 4 or 8) apply;
+ * kernel, 2 fallback, 3 tensor few-token kernel, 4 tensor kernel on half tiles) and "split_k" (parts of the sum: of the few-token
+ * kernel 1, 2, 4 or 8, of the weight gradient 1 to 4) apply;
  * "last_variant", "last_split_k", "last_grid" and "last_tile_n" tell what sgemm_i8_linear and sgemm_i8_wgrad ran. */
 
 /* Linear layer: Y[i, j] = fp32(sum_k W[k, i] * X[k, j]) * x_scale[j] * w_scale[i] (+ bias[i]) for M channels and N tokens, W

@@ -39,7 +39,6 @@ bool i8_view(sgemm_handle *h, I8View *v) {
     v->status = g_status;
     v->sm_count = 148;
     v->tile_n = 256;
-    v->main_threads = 384;
     v->main_smem = 6 * 32768 + 1280;
     v->force_variant = h->force;
     v->split_k = h->split;

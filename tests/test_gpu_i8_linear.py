@@ -14,7 +14,7 @@ from runner import api
 pytestmark = pytest.mark.gpu
 
 KINDS = ["fp32", "fp16", "bf16"]
-AUTO, MAIN, SIMT, FEW = 0, 1, 2, 3
+AUTO, MAIN, SIMT, FEW, HALF = 0, 1, 2, 3, 4
 
 
 @pytest.fixture(scope="module")
@@ -73,7 +73,7 @@ def test_token_counts(r, kind, n):
     check(run(r, *args, kind), *args, kind)
 
 
-@pytest.mark.parametrize("variant", [MAIN, SIMT, FEW])
+@pytest.mark.parametrize("variant", [MAIN, SIMT, FEW, HALF])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (2, 3, 16), (127, 1, 129), (128, 16, 128), (129, 17, 127), (256, 256, 256), (257, 255, 1000),
                                    (1000, 130, 90), (512, 300, 2048), (40, 600, 4097)])
 def test_every_kernel_on_ragged_shapes(r, variant, m, n, k):
@@ -101,13 +101,13 @@ def test_cut_k_gives_the_same_bits(r, parts, n):
 def test_all_kernels_agree_bit_for_bit(r):
     args = problem(700, 333, 1500, 2)
     outs = []
-    for variant in (MAIN, SIMT, FEW):
+    for variant in (MAIN, SIMT, FEW, HALF):
         r.set_option("force_variant", variant)
         outs.append(run(r, *args, "fp32"))
-    assert np.array_equal(outs[0], outs[1]) and np.array_equal(outs[0], outs[2])
+    assert all(np.array_equal(outs[0], out) for out in outs[1:])
 
 
-@pytest.mark.parametrize("variant", [MAIN, SIMT, FEW])
+@pytest.mark.parametrize("variant", [MAIN, SIMT, FEW, HALF])
 def test_largest_k_and_extreme_values_stay_exact(r, variant):
     """K = 131071 of -128 * -128: one below the 32-bit limit."""
     r.set_option("force_variant", variant)
@@ -154,10 +154,11 @@ def test_large_problem_on_a_sample(r):
     """Many tiles per CTA pair: both accumulators and every ring phase are used over and over."""
     m, n, k = 4000, 4100, 1100
     args = problem(m, n, k, 12)
-    got = run(r, *args, "bf16", ldy=4008)
-    assert r.info("last_variant") == MAIN
-    cols = np.arange(0, n, 13)
-    check(got[cols], args[0][cols], args[1][cols], *args[2:], "bf16")
+    for variant in (MAIN, HALF):
+        r.set_option("force_variant", variant)
+        got = run(r, *args, "bf16", ldy=4008)
+        cols = np.arange(0, n, 13)
+        check(got[cols], args[0][cols], args[1][cols], *args[2:], "bf16")
 
 
 def test_concurrent_streams_and_captured_graphs(r):

@@ -105,7 +105,7 @@ def test_handles_of_other_cubins_are_refused(lib, call):
 
 
 def test_forced_tensor_kernels_refuse_what_they_cannot_serve(lib):
-    for force in (1, 3):
+    for force in (1, 3, 4):
         h = lib.seam_handle(1, force, 0)
         assert linear(lib, h, ldw=257) == -6 and linear(lib, h, x=A + 1) == -6 and linear(lib, h, k=0, ldw=16, ldx=16) == -6
         assert wgrad(lib, h, ldg=260) == -6 and wgrad(lib, h, q=A + 8) == -6 and wgrad(lib, h, t=0) == -6
@@ -136,14 +136,23 @@ def test_linear_plans_cover_the_output(lib):
                         assert name == "generated_gemm_simt" and rec.grid == -(-m // 64) * -(-n // 64) and rec.variant == 2
                         continue
                     assert rec.maps == 2 and list(rec.dims) == [k, m, k, n] and list(rec.box)[:3] == [128, 128, 128]
-                    if name == "generated_gemm":
-                        tiles = -(-m // 256) * -(-n // 256)
-                        assert rec.grid == 2 * min(tiles, 74) and rec.box[3] == 128 and rec.threads == 384 and rec.variant == 1
+                    if name in ("generated_gemm", "i8_linear_half"):
+                        tile = 256 if name == "generated_gemm" else 128
+                        tiles = -(-m // 256) * -(-n // tile)
+                        assert rec.grid == 2 * min(tiles, 74) and rec.box[3] == tile // 2 and rec.threads == 384 and rec.smem <= 232448
+                        assert rec.variant == (1 if tile == 256 else 4)
                     else:
                         tile = int(name.rsplit("_", 1)[1])
                         assert rec.parts in (1, 2, 4, 8) and rec.cluster == rec.parts and rec.box[3] == tile and rec.variant == 3
-                        assert rec.grid == -(-m // 128) * -(-n // tile) * rec.parts and rec.threads == 128 and rec.smem <= 232448
-                        assert n > 128 or tile == next(t for t in (16, 32, 64, 128) if n <= t)
+                        assert rec.grid == -(-m // 128) * rec.parts and rec.threads == 128 and rec.smem <= 232448
+                        assert tile == next(t for t in (16, 32, 64, 128) if n <= t) and -(-k // 128) >= (2 * rec.parts if rec.parts > 1 else 1)
+
+
+def test_linear_plans_follow_the_measured_crossings(lib):
+    name = lambda n, m, k: (linear(lib, lib.seam_handle(1, 0, 0), m=m, n=n, k=k), lib.seam_name(last(lib).function).decode())[1]   # noqa: E731
+    assert name(8192, 8192, 8192) == "generated_gemm" and name(1024, 4096, 4096) == "generated_gemm"
+    assert name(509, 4096, 4096) == "i8_linear_half" and name(200, 8192, 8192) == "i8_linear_half"
+    assert name(1, 4096, 4096) == "i8_linear_few_16" and name(23, 8200, 8190) == "i8_linear_few_32" and name(64, 4096, 4096) == "i8_linear_few_64"
 
 
 def test_row_plans_hold_the_row(lib):
