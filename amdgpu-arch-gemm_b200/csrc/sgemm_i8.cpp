@@ -196,6 +196,7 @@ RowForm row_form(int type, const RowArgs &a) {
 }
 
 int launch_rows(sgemm_handle *h, const I8View &v, int base, int type, RowArgs &a, void *stream) {
+    I8Scope scope(h);
     int kernel = 0;
     plan_rows(v, a.k, a.rows, row_form(type, a), &a.tpr, &kernel);
     const uint32_t threads = std::max<uint32_t>(I8_ROW_THREADS, a.tpr), per_block = threads / a.tpr;
@@ -242,6 +243,7 @@ SGEMM_API int sgemm_i8_linear(sgemm_handle *h, const int8_t *dW, const float *dW
     if (!aligned(dY, type_bytes(y_type))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "Y is not aligned to its element type");
     if (!aligned(dWscale, 4) || !aligned(dXscale, 4) || !aligned(dBias, 4))
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "scales and bias are FP32 and must be aligned to 4 bytes");
+    I8Scope scope(h);
     LinearPlan p;
     if ((rc = plan_linear(h, v, dW, dX, m, n, k, ldw, ldx, &p))) return rc;
     LinearArgs a{dW, dWscale, dX, dXscale, dBias, dY, v.status, m, n, k, ldw, ldx, ldy, (uint32_t)y_type, 0, 0};
@@ -310,6 +312,7 @@ SGEMM_API int sgemm_i8_restore(sgemm_handle *h, const int8_t *dQ, const float *d
     const bool vec = aligned(dQ, 16) && ldq % 16 == 0 && aligned(dOut, 16) && (uint64_t)ldo * eb % 16 == 0;
     const uint64_t units = (uint64_t)(vec ? ceil_div(k, 16) : ceil_div(k, 16 / eb) + 1) * n;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((units + 255) / 256, (uint64_t)v.sm_count * 32);
+    I8Scope scope(h);
     void *params[] = {&dQ, &dScale, &dOut, &k, &n, &ldq, &ldo};
     return i8_launch(h, v.functions[kRestore + 2 * out_type + (vec ? 0 : 1)], blocks, 256, 0, 0, stream, params);
 }
@@ -360,6 +363,7 @@ SGEMM_API int sgemm_i8_wgrad(sgemm_handle *h, const int8_t *dQ, const float *dSc
     const bool tma = aligned(dQ, 16) && ldq % 16 == 0 && aligned(dG, 16) && ldg % 8 == 0 && tokens > 0;
     if (v.force_variant != 0 && v.force_variant != 2 && !tma)
         return refuse(h, SGEMM_ERR_UNSUPPORTED, op, "the tensor kernel is forced but the operands need 16-byte aligned bases, ldq a multiple of 16, ldg of 8, and a token");
+    I8Scope scope(h);
     WgradArgs a{dQ, dScale, dG, dC, dD, v.status, m, n, tokens, ldq, ldg, ldc, ldd, (uint32_t)g_type, (uint32_t)d_type, alpha, beta, 0, 0};
     if (!tma || v.force_variant == 2) {
         a.tiles_m = ceil_div(m, I8_SIMT_TILE);

@@ -78,10 +78,21 @@ int i8_wgrad_function();   // index of the weight gradient's kernel, and its blo
 uint32_t i8_wgrad_threads();
 // The words an INT8 cubin carries as `sgemm_i8_layout` when it was compiled from the sources of this library.
 const uint32_t *i8_layout(size_t *words);
-// Launch on the handle's context; cluster: CTAs per cluster (0: as compiled).
+// Make the handle's context current on this thread for the object's life (tensor maps and launches need one; the caller's is put back).
+class I8Scope {
+public:
+    explicit I8Scope(sgemm_handle *h);
+    ~I8Scope();
+    I8Scope(const I8Scope &) = delete;
+    I8Scope &operator=(const I8Scope &) = delete;
+
+private:
+    bool pushed_ = false;
+};
+// Launch (inside an I8Scope); cluster: CTAs per cluster (0: as compiled).
 int i8_launch(sgemm_handle *h, void *function, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, void *stream,
               void **params);
-// 2-D tensor map, dims {d0 (contiguous), d1}, box {b0, b1}, with the 128-byte swizzle or none.
+// 2-D tensor map (inside an I8Scope), dims {d0 (contiguous), d1}, box {b0, b1}, with the 128-byte swizzle or none.
 enum I8MapType { kMapInt8, kMapFp16, kMapBf16 };
 int i8_encode(sgemm_handle *h, I8TensorMap *map, I8MapType type, const void *base, uint64_t d0, uint64_t d1, uint64_t stride_bytes,
               uint32_t b0, uint32_t b1, bool swizzle);

@@ -1532,9 +1532,14 @@ bool i8_view(sgemm_handle *h, I8View *view) {
     return true;
 }
 
+I8Scope::I8Scope(sgemm_handle *h) : pushed_(driver().cuCtxPushCurrent_(h->ctx) == CUDA_SUCCESS) {}
+I8Scope::~I8Scope() {
+    CUcontext c;
+    if (pushed_) driver().cuCtxPopCurrent_(&c);
+}
+
 int i8_launch(sgemm_handle *h, void *function, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, void *stream,
               void **params) {
-    CtxGuard guard(h);
     return launch(h, reinterpret_cast<CUfunction>(function), grid, 1, 1, threads, 1, smem, (CUstream)stream, params, cluster);
 }
 

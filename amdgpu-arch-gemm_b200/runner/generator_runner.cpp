@@ -8,7 +8,9 @@
 // std::random_device, beta comes from SGEMM_BETA (default 1, the reference's hard-coded value), and the
 // time of the single CPU validation run is reported as measured rather than divided by `runs`.  Cubins for FP16 or
 // BF16 operands (an addition; the reference is FP32 only) are driven too: A and B are drawn in FP32, converted on
-// the device, the CPU check runs on the converted values and the SIMT block is printed with zeros.
+// the device, the CPU check runs on the converted values and the SIMT block is printed with zeros.  Cubins for INT8
+// operands run the 8-bit linear layer: both operands are drawn in FP32 (A as K x M, B as K x N), quantised on the device with one scale
+// per channel and token, multiplied into an FP32 D, and checked against the CPU's integer sums; beta does not apply.
 //
 // Extra diagnostics go to stderr so the stdout contract stays intact; with SGEMM_JSON=<path> the measured block is
 // also written to that file as one JSON object (shape, variant, split-K, ms, TFLOP/s, GiB/s figure, mismatches).
@@ -124,6 +126,98 @@ int on_all_gpus(F work) {
     return 0;
 }
 
+// The INT8 cubin's run: the same stdout blocks for D[i, j] = sx[j] * sw[i] * sum_k W[k, i] X[k, j].
+int run_int8(const char *cubin, const char *toml, int device, uint32_t m, uint32_t n, uint32_t k, uint32_t warmup, uint32_t runs,
+             bool validate, uint64_t seed) {
+    g_ranks.resize(1);
+    int rc = sgemm_open(cubin, toml, device, &g_ranks[0].h);
+    if (rc) return die(nullptr, "sgemm_open", rc);
+    sgemm_handle *h = g_ranks[0].h;
+    const uint32_t pitch = (k + 15) / 16 * 16;   // whole 16-byte units: what the tensor-core kernels read
+    const size_t nw = (size_t)m * k, nx = (size_t)n * k, ny = (size_t)m * n;
+    void *w32 = nullptr, *x32 = nullptr, *w = nullptr, *x = nullptr, *sw = nullptr, *sx = nullptr, *y = nullptr;
+    struct { void **p; size_t bytes; } buffers[] = {{&w32, nw * 4}, {&x32, nx * 4}, {&w, (size_t)m * pitch}, {&x, (size_t)n * pitch},
+                                                    {&sw, (size_t)m * 4}, {&sx, (size_t)n * 4}, {&y, ny * 4}};
+    for (auto &b : buffers)
+        if ((rc = sgemm_dev_alloc(h, b.bytes, b.p))) return die(h, "device allocation", rc);
+    if ((rc = sgemm_fill_uniform(h, (float *)w32, nw, 0, seed, nullptr)) || (rc = sgemm_fill_uniform(h, (float *)x32, nx, 0, seed + 1, nullptr)) ||
+        (rc = sgemm_i8_quantize(h, w32, 0, (int8_t *)w, (float *)sw, k, m, k, pitch, 0, nullptr)) ||
+        (rc = sgemm_i8_quantize(h, x32, 0, (int8_t *)x, (float *)sx, k, n, k, pitch, 0, nullptr)) || (rc = sgemm_dev_sync(h)))
+        return die(h, "input fill and quantisation", rc);
+    std::vector<float> cpu_y;
+    if (validate) {
+        std::vector<int8_t> hw((size_t)m * pitch), hx((size_t)n * pitch);
+        std::vector<float> hsw(m), hsx(n);
+        if ((rc = sgemm_dev_download(h, hw.data(), w, hw.size())) || (rc = sgemm_dev_download(h, hx.data(), x, hx.size())) ||
+            (rc = sgemm_dev_download(h, hsw.data(), sw, (size_t)m * 4)) || (rc = sgemm_dev_download(h, hsx.data(), sx, (size_t)n * 4)))
+            return die(h, "input download", rc);
+        cpu_y.resize(ny);
+        const auto t0 = std::chrono::steady_clock::now();
+#pragma omp parallel for schedule(dynamic, 4)
+        for (int64_t j = 0; j < (int64_t)n; ++j)
+            for (uint32_t i = 0; i < m; ++i) {
+                int32_t acc = 0;
+                const int8_t *pw = hw.data() + (size_t)i * pitch, *px = hx.data() + (size_t)j * pitch;
+                for (uint32_t l = 0; l < k; ++l) acc += (int32_t)pw[l] * px[l];
+                cpu_y[i + (size_t)j * m] = (float)acc * hsx[j] * hsw[i];
+            }
+        const auto t1 = std::chrono::steady_clock::now();
+        std::cout << "cpuGemm func: " << std::chrono::duration<float, std::milli>(t1 - t0).count() << " ms\n";
+    }
+    auto bench = [&](int force_variant, float *ms) -> int {
+        int e = sgemm_set_option(h, "force_variant", force_variant);
+        std::chrono::steady_clock::time_point t0;
+        for (uint32_t i = 0; !e && i < warmup + runs; ++i) {
+            if (i == warmup) {
+                e = sgemm_dev_sync(h);
+                t0 = std::chrono::steady_clock::now();
+            }
+            if (!e) e = sgemm_i8_linear(h, (const int8_t *)w, (const float *)sw, (const int8_t *)x, (const float *)sx, nullptr, y, 0, m, n, k, pitch, pitch, m, nullptr);
+        }
+        if (!e) e = sgemm_dev_sync(h);
+        *ms = std::chrono::duration<float, std::milli>(std::chrono::steady_clock::now() - t0).count() / (float)runs;
+        return e;
+    };
+    auto gibs = [&](float ms) { return ((float)nw + (float)nx + 4.0f * (float)ny) / ms * 1e3f / 1024.f / 1024.f / 1024.f; };
+    float ms = 0.f;
+    if ((rc = bench(2, &ms))) return die(h, "SIMT comparison run", rc);
+    std::cout << "SIMT gemm: " << ms << " ms\nGflops: " << gflops(m, n, k, ms) << "\nGiB/s: " << gibs(ms) << '\n';
+    if ((rc = sgemm_dev_memset(h, y, 0, ny * 4)) || (rc = bench(0, &ms))) return die(h, "measured run", rc);
+    uint32_t status[8];
+    if ((rc = sgemm_last_status(h, status))) return die(h, "device status check", rc);
+    int64_t variant = 0, parts = 1;
+    sgemm_get_info(h, "last_variant", &variant);
+    sgemm_get_info(h, "last_split_k", &parts);
+    std::fprintf(stderr, "measured kernel: %s, split_k %lld, %.3f TOPS\n", variant == 2 ? "SIMT dp4a" : "tcgen05 INT8", (long long)parts,
+                 gflops(m, n, k, ms) * 1e-3);
+    std::cout << "ASM gemm: " << ms << " ms\nGflops: " << gflops(m, n, k, ms) << "\nGiB/s: " << gibs(ms) << '\n';
+    size_t mismatches = 0;
+    if (validate) {
+        std::vector<float> gpu_y(ny);
+        if ((rc = sgemm_dev_download(h, gpu_y.data(), y, ny * 4))) return die(h, "result download", rc);
+        for (size_t i = 0; i < ny; ++i)
+            if (!(std::fabs(gpu_y[i] - cpu_y[i]) < 1e-3f)) {
+                if (mismatches++ < 10) std::cout << "gpu & cpu results mismatched at index: " << i << '\n' << gpu_y[i] << " != " << cpu_y[i] << '\n';
+            }
+        std::cout << "# of mismatches: " << mismatches << "/" << ny << '\n';
+    }
+    if (const char *json_path = std::getenv("SGEMM_JSON")) {
+        if (FILE *f = std::fopen(json_path, "w")) {
+            std::fprintf(f, "{\"m\": %u, \"n\": %u, \"k\": %u, \"seed\": %llu, \"warmup\": %u, \"runs\": %u, \"variant\": \"%s\", \"split_k\": %lld, "
+                            "\"ms\": %.6f, \"tflops\": %.4f, \"gib_per_s\": %.3f, \"validated\": %s, \"mismatches\": %zu, \"ngpus\": 1}\n",
+                         m, n, k, (unsigned long long)seed, warmup, runs, variant == 2 ? "simt_dp4a" : "tcgen05_int8", (long long)parts, ms,
+                         gflops(m, n, k, ms) * 1e-3, gibs(ms), validate ? "true" : "false", mismatches);
+            std::fclose(f);
+        } else {
+            std::fprintf(stderr, "GeneratorRunner: cannot write %s\n", json_path);
+        }
+    }
+    for (auto &b : buffers) sgemm_dev_free(h, *b.p);
+    sgemm_close(h);
+    g_ranks.clear();
+    return mismatches ? -1 : 0;
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -157,6 +251,17 @@ int main(int argc, char **argv) {
     // FP32 like everything else here and converted on the device; the CPU check runs on the converted values
     sgemm_config parsed;
     const bool half = sgemm_config_parse(argv[2], &parsed) == 0 && parsed.a_type != 0;
+    if (half && parsed.a_type == 3) {
+        if (ngpus > 1 || allgather) {
+            std::fprintf(stderr, "GeneratorRunner: INT8 cubins run on one GPU\n");
+            return 3;
+        }
+        if (k > 131071) {
+            std::fprintf(stderr, "GeneratorRunner: K above 131071: the 32-bit integer sum could overflow\n");
+            return -1;
+        }
+        return run_int8(argv[1], argv[2], device, m, n, k, warmup, runs, validate, seed);
+    }
     if (half && (parsed.trans_a || parsed.trans_b)) {
         std::fprintf(stderr, "GeneratorRunner: %s describes a 16-bit kernel for transposed operands; this program drives the NN layout\n", argv[2]);
         return 2;

@@ -22,6 +22,7 @@ sgemm_handle g_handle;
 Launch g_last;
 std::string g_error;
 uint32_t g_maps = 0;
+int g_scopes = 0;   // contexts made current and not put back
 void *g_functions[sgemm_internal::kI8Functions];
 uint32_t g_status[16];
 }  // namespace
@@ -46,7 +47,11 @@ bool i8_view(sgemm_handle *h, I8View *v) {
     for (int i = 0; i < 5; ++i) v->wgrad_clusters[i] = fit[i];
     return true;
 }
+I8Scope::I8Scope(sgemm_handle *) : pushed_(true) { ++g_scopes; }
+I8Scope::~I8Scope() { g_scopes -= pushed_; }
+
 int i8_launch(sgemm_handle *, void *function, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, void *, void **params) {
+    if (g_scopes != 1) return -4;   // as the driver: no current context
     ++g_last.count;
     g_last.function = (int32_t)(reinterpret_cast<uintptr_t>(function) - 1);
     g_last.grid = grid;
@@ -62,6 +67,7 @@ int i8_launch(sgemm_handle *, void *function, uint32_t grid, uint32_t threads, u
     return 0;
 }
 int i8_encode(sgemm_handle *, I8TensorMap *, I8MapType, const void *, uint64_t d0, uint64_t d1, uint64_t, uint32_t b0, uint32_t b1, bool) {
+    if (g_scopes != 1) return -4;
     if (g_maps < 2) {
         g_last.dims[2 * g_maps] = d0;
         g_last.dims[2 * g_maps + 1] = d1;
