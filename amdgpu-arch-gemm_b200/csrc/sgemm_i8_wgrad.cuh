@@ -20,9 +20,9 @@
 // Both operands are MN-major 16-bit tiles (a row of 128 bytes = 64 features or channels of one token, 128-byte swizzle,
 // repeating unit 8 tokens: SBO = 1024; chunks of 64 features I8W_BK * 128 bytes apart: LBO); one MMA takes 16 tokens = 2048 bytes.
 //
-// The tensor core adds to its accumulator with truncation, so a long sum drifts toward zero: every I8W_CHAIN stages (the first two
-// chains of a tile are twice as long) the issuer turns to the other TMEM buffer and the epilogue warps add the finished chain to
-// a running sum in registers, rounding to nearest, in a fixed order.
+// The tensor core adds to its accumulator with truncation, so a long sum drifts toward zero: every I8W_CHAIN stages (32 additions) the
+// issuer turns to the other TMEM buffer and the epilogue warps add the finished chain to a running sum in registers, rounding to
+// nearest, in a fixed order.
 //
 // Few tiles and many tokens: S = 2, 3 or 4 pairs of a cluster take S parts of the tokens of one tile.  Each leaves its sums in
 // its shared memory and after a cluster barrier adds up its share of the columns over all parts, in the order of the
@@ -62,7 +62,6 @@ __device__ __forceinline__ uint32_t i8w_idesc(uint32_t g_type) {
     const uint32_t fmt = g_type == SGEMM_I8_BF16 ? 1u : 0u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 }
-__device__ __forceinline__ uint32_t i8w_chain_span(uint32_t blocks_done) { return blocks_done < 4u * I8W_CHAIN ? 2u * I8W_CHAIN : I8W_CHAIN; }
 
 // two values to one word of G's type, round to nearest even
 __device__ __forceinline__ uint32_t i8w_pack(float lo, float hi, uint32_t g_type) {
@@ -289,7 +288,7 @@ i8_wgrad(const __grid_constant__ I8WgradArgs a, const __grid_constant__ I8Tensor
                         const uint32_t buf = handover & 1u, acc_phase = (handover >> 1) & 1u;
                         if (!i8_wait_warp(waiter, bar_tempty + 8 * buf, acc_phase ^ 1u, 0x220u + buf, tile, kb)) { alive = false; break; }
                         i8_fence_after();
-                        const uint32_t chain_begin = kb, chain_end = min(kb_end, kb + i8w_chain_span(kb - kb_begin));
+                        const uint32_t chain_begin = kb, chain_end = min(kb_end, kb + I8W_CHAIN);
                         for (; kb < chain_end; ++kb) {
                             // (a widened tile's "ready" implies that both CTAs' G tiles have landed)
                             if (!i8_wait_warp(waiter, bar_ready + 8 * widened, phase, 0x320u + widened, tile, kb)) { alive = false; break; }
@@ -390,7 +389,7 @@ i8_wgrad(const __grid_constant__ I8WgradArgs a, const __grid_constant__ I8Tensor
                 else i8w_add_c<SGEMM_I8_FP16>(sum2, a, row, row_first, col0);
             }
             const uint64_t alpha2 = i8w_pair(a.alpha, a.alpha);
-            for (uint32_t kb = kb_begin; kb < kb_end; kb += i8w_chain_span(kb - kb_begin), ++handover) {
+            for (uint32_t kb = kb_begin; kb < kb_end; kb += I8W_CHAIN, ++handover) {
                 const uint32_t buf = handover & 1u, acc_phase = (handover >> 1) & 1u;
                 alive = i8_wait_warp(waiter, bar_tfull + 8 * buf, acc_phase, 0x420u + buf, tile, kb);
                 if (!alive) break;
