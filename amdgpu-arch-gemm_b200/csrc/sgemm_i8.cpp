@@ -94,6 +94,8 @@ int begin(sgemm_handle *h, const char *op, I8View *v) {
 
 constexpr uint32_t kLargest = 0x7FFFFF00u;   // sizes above this would leave 31 bits when rounded up to a tile
 
+constexpr uint32_t kLongestRow = 1u << 30;   // the row kernels count a row's elements in 32 bits with a sign
+
 // ---------------------------------------------------------------------------------------------- linear
 struct LinearPlan {
     int index = kLinear;
@@ -287,7 +289,7 @@ SGEMM_API int sgemm_i8_quantize(sgemm_handle *h, const void *dX, int x_type, int
     if (ldx < std::max(k, 1u) || ldq < std::max(k, 1u))
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a leading dimension is smaller than the rows it must hold");
     if (n == 0) return SGEMM_OK;
-    if (k > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (k > kLongestRow || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
     if (!dScale || (k && (!dX || !dQ))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X, Q or the scales are NULL");
     const uint32_t eb = type_bytes(x_type);
     if (!aligned(dX, eb) || !aligned(dScale, 4)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X or the scales are not aligned to their element type");
@@ -330,7 +332,7 @@ SGEMM_API int sgemm_i8_rmsnorm(sgemm_handle *h, const void *dX, const void *dRes
     if (ldx < k || ldq < k || (dResidual && ldr < k) || (dSum && lds < k))
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a leading dimension is smaller than the rows it must hold");
     if (n == 0) return SGEMM_OK;
-    if (k > kLargest || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
+    if (k > kLongestRow || n > kLargest) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "problem too large");
     if (!dX || !dGamma || !dQ || !dScale) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X, gamma, Q or the scales are NULL");
     const uint32_t eb = type_bytes(x_type);
     if (!aligned(dX, eb) || !aligned(dGamma, eb) || !aligned(dResidual, eb) || !aligned(dSum, eb) || !aligned(dScale, 4))

@@ -11,7 +11,7 @@
 
 namespace {
 
-PyObject *s_data_ptr, *s_get_device, *s_dtype, *s_is_contiguous, *s_addr;   // interned names
+PyObject *s_data_ptr, *s_get_device, *s_dtype, *s_is_contiguous, *s_addr, *s_stride, *s_shape;   // interned names
 PyObject *g_codes = nullptr;       // dtype object -> type code (api._type_codes)
 PyObject *g_type_code = nullptr;   // api._type_code
 
@@ -89,10 +89,39 @@ struct Call {
         }
         return (uint32_t)v;
     }
-    // a leading dimension, 0: the columns lie one behind the other
-    uint32_t ld(PyObject *x, uint32_t rows) {
-        const uint32_t v = u32(x);
-        return v ? v : rows ? rows : 1u;
+    // A leading dimension.  0: the row pitch of a tensor of two or more dimensions, else the columns lie one behind the other.
+    uint32_t ld(PyObject *given, PyObject *matrix, uint32_t rows) {
+        const uint32_t v = u32(given), dense = rows ? rows : 1u;
+        if (!ok || v || matrix == Py_None || PyLong_CheckExact(matrix)) return v ? v : dense;
+        PyObject *r = PyObject_CallMethodNoArgs(matrix, s_stride);   // a tuple; an object without one is dense
+        if (!r) {
+            PyErr_Clear();
+            return dense;
+        }
+        uint32_t pitch = dense;
+        if (PyTuple_Check(r) && PyTuple_GET_SIZE(r) >= 2) {
+            const long long stride = PyLong_AsLongLong(PyTuple_GET_ITEM(r, PyTuple_GET_SIZE(r) - 2));
+            if (stride >= (long long)dense && stride <= 0xFFFFFFFFll) pitch = (uint32_t)stride;
+            else if (one_row(matrix)) pitch = dense;   // (the stride of a dimension of one says nothing)
+            else {
+                PyErr_Format(PyExc_ValueError, "a tensor's rows are %lld elements apart, the call reads %u of each", stride, dense);
+                ok = false;
+            }
+        }
+        Py_DECREF(r);
+        return pitch;
+    }
+    bool one_row(PyObject *matrix) {
+        PyObject *shape = PyObject_GetAttr(matrix, s_shape);
+        bool one = false;
+        if (shape && PySequence_Check(shape) && PySequence_Size(shape) >= 2) {
+            PyObject *rows = PySequence_GetItem(shape, PySequence_Size(shape) - 2);
+            one = rows && PyLong_AsLong(rows) <= 1;
+            Py_XDECREF(rows);
+        }
+        Py_XDECREF(shape);
+        PyErr_Clear();
+        return one;
     }
     float f32(PyObject *x) {
         if (!ok) return 0.0f;
@@ -138,7 +167,7 @@ NATIVE_BEGIN(i8_linear, 14)
     void *y = c.addr(a[4], "y", -1);
     const uint32_t m = c.u32(a[5]), tokens = c.u32(a[6]), k = c.u32(a[7]);
     const auto *bias = static_cast<const float *>(c.addr(a[8], "bias", 0));
-    const uint32_t ldw = c.ld(a[9], k), ldx = c.ld(a[10], k), ldy = c.ld(a[11], m);
+    const uint32_t ldw = c.ld(a[9], a[0], k), ldx = c.ld(a[10], a[2], k), ldy = c.ld(a[11], a[4], m);
     const int type = c.type(a[4], a[12]);
     void *stream = c.ptr(a[13]);
 NATIVE_END(sgemm_i8_linear(h, w, ws, x, xs, bias, y, type, m, tokens, k, ldw, ldx, ldy, stream))
@@ -150,7 +179,7 @@ NATIVE_BEGIN(i8_quantize, 10)
     auto *s = static_cast<float *>(c.addr(a[2], "scale", 0));
     const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]);
     const int pow2 = c.flag(a[5]);
-    const uint32_t ldx = c.ld(a[6], k), ldq = c.ld(a[7], k);
+    const uint32_t ldx = c.ld(a[6], a[0], k), ldq = c.ld(a[7], a[1], k);
     const int type = c.type(a[0], a[8]);
     void *stream = c.ptr(a[9]);
 NATIVE_END(sgemm_i8_quantize(h, x, type, q, s, k, rows, ldx, ldq, pow2, stream))
@@ -160,7 +189,7 @@ NATIVE_BEGIN(i8_restore, 9)
     const auto *q = static_cast<const int8_t *>(c.addr(a[0], "q", 3));
     const auto *s = static_cast<const float *>(c.addr(a[1], "scale", 0));
     void *out = c.addr(a[2], "out", -1);
-    const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]), ldq = c.ld(a[5], k), ldo = c.ld(a[6], k);
+    const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]), ldq = c.ld(a[5], a[0], k), ldo = c.ld(a[6], a[2], k);
     const int type = c.type(a[2], a[7]);
     void *stream = c.ptr(a[8]);
 NATIVE_END(sgemm_i8_restore(h, q, s, out, type, k, rows, ldq, ldo, stream))
@@ -176,7 +205,7 @@ NATIVE_BEGIN(i8_rmsnorm, 15)
     const void *res = c.addr(a[6], "residual", same);
     void *sum = c.addr(a[7], "sum_out", same);
     const float eps = c.f32(a[8]);
-    const uint32_t ldx = c.ld(a[9], k), ldr = c.ld(a[10], k), ldq = c.ld(a[11], k), lds = c.ld(a[12], k);
+    const uint32_t ldx = c.ld(a[9], a[0], k), ldr = c.ld(a[10], a[6], k), ldq = c.ld(a[11], a[2], k), lds = c.ld(a[12], a[7], k);
     void *stream = c.ptr(a[14]);
 NATIVE_END(sgemm_i8_rmsnorm(h, x, res, g, type, eps, q, s, sum, k, rows, ldx, ldr, ldq, lds, stream))
 
@@ -190,7 +219,7 @@ NATIVE_BEGIN(i8_wgrad, 17)
     const int dy_type = c.type(a[2], a[14]), dw_type = c.type(a[3], a[15]);
     const void *prior = c.addr(a[7], "c", a[15] == Py_None ? dw_type : -1);
     const float alpha = c.f32(a[8]), beta = c.f32(a[9]);
-    const uint32_t ldq = c.ld(a[10], m), lddy = c.ld(a[11], channels), ldc = c.ld(a[12], m), lddw = c.ld(a[13], m);
+    const uint32_t ldq = c.ld(a[10], a[0], m), lddy = c.ld(a[11], a[2], channels), ldc = c.ld(a[12], a[7], m), lddw = c.ld(a[13], a[3], m);
     void *stream = c.ptr(a[16]);
 NATIVE_END(sgemm_i8_wgrad(h, q, s, dy, dy_type, prior, dw, dw_type, alpha, beta, m, channels, tokens, ldq, lddy, ldc, lddw, stream))
 
@@ -221,6 +250,8 @@ PyMODINIT_FUNC PyInit__sgemm_native(void) {
     s_dtype = PyUnicode_InternFromString("dtype");
     s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
     s_addr = PyUnicode_InternFromString("_addr");
-    if (!s_data_ptr || !s_get_device || !s_dtype || !s_is_contiguous || !s_addr) return nullptr;
+    s_stride = PyUnicode_InternFromString("stride");
+    s_shape = PyUnicode_InternFromString("shape");
+    if (!s_stride || !s_shape || !s_data_ptr || !s_get_device || !s_dtype || !s_is_contiguous || !s_addr) return nullptr;
     return PyModule_Create(&g_module);
 }

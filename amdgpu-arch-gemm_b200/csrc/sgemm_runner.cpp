@@ -1425,6 +1425,7 @@ SGEMM_API int sgemm_fill_uniform(sgemm_handle *h, float *dptr, uint64_t count, u
 
 SGEMM_API int sgemm_narrow16(sgemm_handle *h, const float *dsrc, void *ddst, uint64_t count, void *stream) {
     if (!h || ((!dsrc || !ddst) && count)) return SGEMM_ERR_INVALID_ARGUMENT;
+    if (h->elem_bytes == 1) return refuse_i8(h);
     if (h->elem_bytes != 2)
         return fail(h, SGEMM_ERR_UNSUPPORTED, "sgemm_narrow16 converts to the operand type of a cubin for FP16 or BF16 operands; this one takes FP32");
     if (count == 0) return SGEMM_OK;

@@ -128,7 +128,7 @@ def test_tensors_of_the_wrong_kind_are_refused(r):
     with pytest.raises(OverflowError):
         r.i8_linear(q, s, q, s, y, 16, 2 ** 32, 32)
     with pytest.raises(api.SgemmError, match="K above 131071"):
-        r.i8_linear(q, s, q, s, y, 16, 16, 131072)
+        r.i8_linear(q, s, q, s, y, 16, 16, 131072, ldw=131072, ldx=131072)
     with pytest.raises(api.SgemmError, match="leading dimension"):
         r.i8_linear(q, s, q, s, y, 16, 16, 32, ldw=31)
     x16 = torch.zeros(64 * 64, device="cuda")
@@ -136,6 +136,23 @@ def test_tensors_of_the_wrong_kind_are_refused(r):
         r.launch(x16, x16, None, x16, 8, 8, 8)
     with pytest.raises(api.SgemmError, match="sgemm_i8"):
         r.workspace_bytes(256, 256, 256)
+
+
+def test_leading_dimensions_come_from_two_dimensional_tensors(r):
+    """Rows inside wider buffers without a leading dimension in the call; rows that overlap are refused."""
+    rng = np.random.default_rng(2)
+    x = tensor(rng.standard_normal((20, 96)), torch.float32)
+    q, s, out = torch.zeros(20, 64, dtype=torch.int8, device="cuda"), torch.zeros(20, device="cuda"), torch.zeros(20, 80, device="cuda")
+    r.i8_quantize(x[:, :50], q[:, :50], s, 50, 20)
+    r.i8_restore(q, s, out[:, 3:53], 50, 20)
+    torch.cuda.synchronize()
+    want, scale = model.quantize(x.double().cpu().numpy()[:, :50])
+    assert np.array_equal(q.cpu().numpy()[:, :50], want) and (q[:, 50:] == 0).all()
+    assert np.array_equal(out[:, 3:53].double().cpu().numpy(), model.restore(want, s.double().cpu().numpy(), "fp32"))
+    assert (out[:, :3] == 0).all() and (out[:, 53:] == 0).all()
+    with pytest.raises(ValueError, match="apart"):
+        r.i8_quantize(x[:1].expand(20, 96), q, s, 50, 20)
+    r.i8_quantize(x[:1].expand(1, 96), q, s, 50, 1)
 
 
 def test_other_cubins_refuse_the_8_bit_calls(built):
