@@ -71,8 +71,8 @@ struct WgradArgs {
 struct RowArgs {
     const void *x, *r, *g;
     void *sum, *q, *scale;
-    uint32_t k, rows, ldx, ldr, lds, ldq, tpr, pow2;
-    float eps;
+    uint32_t k, rows, ldx, ldr, lds, ldq, tpr, tpr_log2, passes, pow2;
+    float eps, inv_k;
 };
 
 int refuse(sgemm_handle *h, int code, const char *op, const char *what) {
@@ -200,7 +200,13 @@ RowForm row_form(int type, const RowArgs &a) {
 int launch_rows(sgemm_handle *h, const I8View &v, int base, int type, RowArgs &a, void *stream) {
     I8Scope scope(h);
     int kernel = 0;
-    plan_rows(v, a.k, a.rows, row_form(type, a), &a.tpr, &kernel);
+    const RowForm form = row_form(type, a);
+    plan_rows(v, a.k, a.rows, form, &a.tpr, &kernel);
+    const uint32_t span = a.tpr * (kernel == 0 ? 8 : kernel == 1 ? 16 : 32);
+    const uint32_t reach = a.k + (form == kRowsShifted ? 16 / type_bytes(type) - 1 : 0);   // of a shifted row from its first vector on
+    a.passes = std::max(1u, ceil_div(reach, span));
+    for (a.tpr_log2 = 0; (1u << a.tpr_log2) < a.tpr;) ++a.tpr_log2;
+    a.inv_k = a.k ? 1.0f / (float)a.k : 0.0f;
     const uint32_t threads = std::max<uint32_t>(I8_ROW_THREADS, a.tpr), per_block = threads / a.tpr;
     void *params[] = {&a};
     return i8_launch(h, v.functions[base + 5 * type + kernel], ceil_div(a.rows, per_block), threads, 0, 0, stream, params);
@@ -293,7 +299,7 @@ SGEMM_API int sgemm_i8_quantize(sgemm_handle *h, const void *dX, int x_type, int
     if (!dScale || (k && (!dX || !dQ))) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X, Q or the scales are NULL");
     const uint32_t eb = type_bytes(x_type);
     if (!aligned(dX, eb) || !aligned(dScale, 4)) return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "X or the scales are not aligned to their element type");
-    RowArgs a{dX, nullptr, nullptr, nullptr, dQ, dScale, k, n, ldx, 0, 0, ldq, 32, (uint32_t)pow2, 0.0f};
+    RowArgs a{dX, nullptr, nullptr, nullptr, dQ, dScale, k, n, ldx, 0, 0, ldq, 32, 0, 0, (uint32_t)pow2, 0.0f, 0.0f};
     return launch_rows(h, v, kQuantize, x_type, a, stream);
 }
 
@@ -339,7 +345,7 @@ SGEMM_API int sgemm_i8_rmsnorm(sgemm_handle *h, const void *dX, const void *dRes
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "a matrix is not aligned to its element type");
     if ((dSum == dX && dX && lds != ldx) || (dSum == dResidual && dSum && lds != ldr))
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "the sum may replace X or the residual only with the same leading dimension");
-    RowArgs a{dX, dResidual, dGamma, dSum, dQ, dScale, k, n, ldx, ldr, lds, ldq, 32, 0, eps};
+    RowArgs a{dX, dResidual, dGamma, dSum, dQ, dScale, k, n, ldx, ldr, lds, ldq, 32, 0, 0, 0, eps, 0.0f};
     return launch_rows(h, v, kNorm, x_type, a, stream);
 }
 

@@ -53,6 +53,6 @@
             I8_SIMT_THREADS, I8_ROW_THREADS, SGEMM_I8_ARGS_VERSION                                                         \
     }
 #define SGEMM_I8_LAYOUT_WORDS 16
-#define SGEMM_I8_ARGS_VERSION 1   // raised with every change of an argument structure
+#define SGEMM_I8_ARGS_VERSION 2   // raised with every change of an argument structure
 
 #endif

@@ -40,8 +40,9 @@ struct I8RowArgs {
     float *scale;
     uint32_t k, rows, ldx, ldr, lds, ldq;
     uint32_t tpr;         // threads per row, a power of two, 32 .. 1024 (PER 8), 512 (16) or 256 (32)
+    uint32_t tpr_log2, passes;   // how often tpr * PER elements take a row (host: an integer division is 30 instructions)
     uint32_t pow2;
-    float eps;
+    float eps, inv_k;
 };
 
 __device__ __forceinline__ uint32_t i8_abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
@@ -188,10 +189,11 @@ __device__ __forceinline__ I8Rounding i8_rounding(uint32_t peak_bits, bool pow2,
     return r;
 }
 
+// rsqrt(mean + eps): the product with 1 / K is off by 2^-23 and rsqrtf by 2 of its last places
 template <uint32_t TYPE>
-__device__ __forceinline__ float i8_rstd(const float (&sums)[2], uint32_t k, float eps) {
-    if (TYPE != SGEMM_I8_FP16 && !(sums[0] < INFINITY)) return 0x1p-64f * __frcp_rn(__fsqrt_rn(__fdiv_rn(sums[1], (float)k)));
-    return __frcp_rn(__fsqrt_rn(__fdiv_rn(sums[0], (float)k) + eps));
+__device__ __forceinline__ float i8_rstd(const float (&sums)[2], float inv_k, float eps) {
+    if (TYPE != SGEMM_I8_FP16 && !(sums[0] < INFINITY)) return 0x1p-64f * rsqrtf(sums[1] * inv_k);
+    return rsqrtf(fmaf(sums[0], inv_k, eps));
 }
 
 // The row's peak over its `tpr` threads (and its sums, in a fixed order).
@@ -232,7 +234,7 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
     constexpr int VE = 16 / (int)sizeof(T), NV = PER / VE;
     sgemm_launch_dependents();
     sgemm_grid_dependency_wait();
-    const uint32_t row = blockIdx.x * (blockDim.x / a.tpr) + threadIdx.x / a.tpr, t = threadIdx.x & (a.tpr - 1);
+    const uint32_t row = blockIdx.x * (blockDim.x >> a.tpr_log2) + (threadIdx.x >> a.tpr_log2), t = threadIdx.x & (a.tpr - 1);
     const bool live = row < a.rows;
     const uint64_t r64 = live ? row : 0u;
     const T *x = static_cast<const T *>(a.x) + r64 * a.ldx;
@@ -243,7 +245,7 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
     int8_t *q = a.q + r64 * a.ldq;
     const int32_t k = live ? (int32_t)a.k : 0;
     const uint32_t span = a.tpr * PER;
-    const uint32_t passes = a.k ? (a.k + (SHIFTED ? VE - 1 : 0) + span - 1) / span : 1u;
+    const uint32_t passes = a.passes;
 
     // first element of the thread's i-th vector (negative before the row), and whether the vector lies inside the row
     auto first = [&](uint32_t pass, int i) -> int32_t { return (int32_t)(pass * span + (i * a.tpr + t) * VE) - off; };
@@ -344,7 +346,7 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
     if (!live) return;   // (a warp has one row: tpr is at least 32)
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (NORM) scale *= i8_rstd<TYPE>(sums, a.k, a.eps);
+    if (NORM) scale *= i8_rstd<TYPE>(sums, a.inv_k, a.eps);
     if (t == 0) a.scale[row] = scale;
 
     for (uint32_t pass = 0; pass < passes; ++pass) {
@@ -410,7 +412,7 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
     constexpr int PER = 32;
     sgemm_launch_dependents();
     sgemm_grid_dependency_wait();
-    const uint32_t row = blockIdx.x * (blockDim.x / a.tpr) + threadIdx.x / a.tpr, t = threadIdx.x & (a.tpr - 1);
+    const uint32_t row = blockIdx.x * (blockDim.x >> a.tpr_log2) + (threadIdx.x >> a.tpr_log2), t = threadIdx.x & (a.tpr - 1);
     const bool live = row < a.rows;
     const uint64_t r64 = live ? row : 0u;
     const T *x = static_cast<const T *>(a.x) + r64 * a.ldx;
@@ -419,7 +421,7 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
     T *sum = NORM && a.sum ? static_cast<T *>(a.sum) + r64 * a.lds : nullptr;
     int8_t *q = a.q + r64 * a.ldq;
     const uint32_t k = live ? a.k : 0u, span = a.tpr * PER;
-    const uint32_t passes = a.k ? (a.k + span - 1) / span : 1u;
+    const uint32_t passes = a.passes;
     float p[PER];
     float sums[2] = {0.0f, 0.0f};
     uint32_t peak_bits = 0u;
@@ -460,7 +462,7 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
     if (!live) return;
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (NORM) scale *= i8_rstd<TYPE>(sums, a.k, a.eps);
+    if (NORM) scale *= i8_rstd<TYPE>(sums, a.inv_k, a.eps);
     if (t == 0) a.scale[row] = scale;
     for (uint32_t pass = 0; pass < passes; ++pass) {
         if (passes > 1) fetch(pass, true);

@@ -2,9 +2,9 @@
 
 q has to equal the definition's integers.  Scales: max|x| is exact, so max|x| / 127 is one rounding (2^-24); a power of two
 is exact.  The norm's scale has the rounding of P / 127, of the mean (a sum of K squares: each addition rounds to 2^-24 of a
-partial sum that is no larger than the total; a thread adds at most 32 squares to a row, a warp 5 and a block 5 more sums, times K / 32768 + 1 passes),
-of the division by K and the addition of eps, of the square root and the reciprocal, and of the product: below
-(32 + 10 + 8) * 2^-24 for rows of one pass, as the square root halves the sum's share."""
+partial sum that is no larger than the total; a thread adds at most 32 squares of a pass, then a pass's sum to the others', a warp 5 and a
+block 5 more sums), of the product with 1 / K (2^-23) and the addition of eps, all halved by the root, then of rsqrtf (2 last places:
+2^-22) and of the product: (32 + 16 passes + 10 + 3) / 2 + 4 + 2 times 2^-24, below the (50 + 16 passes) * 2^-24 the tests allow."""
 import numpy as np
 import pytest
 import torch
