@@ -10,12 +10,15 @@
 // activations exists in shared memory only: the checkpoint is read as 8 bits.
 //
 // Roles, as in the in-kernel split of the FP32 kernel: a TMA producer brings a stage of I8W_BK tokens (raw int8 tile, G tile), a
-// second warp their scales (4-byte asynchronous copies: any base; fetched by the widening warps themselves they would cost every
-// stage a trip to memory: 1.2 us a stage instead of 0.3);
-// two groups of eight warps, taking stages in turn, widen the raw tile into an A operand; one thread of the pair's leader
-// issues the MMAs; eight warps drain the accumulators.  CTA pairs (cta_group::2) work on 256 features x 256 channels: each CTA widens 128 features and
-// stages 128 channels, so a widened element meets 256 channels and the widening (8192 elements a stage) hides beside the
-// stage's 512 tensor cycles.
+// second warp their scales (4-byte asynchronous copies: any base, and no trip to memory inside the widening warps); two groups of
+// eight warps, taking stages in turn, widen the raw tile into an A operand; one thread of the pair's leader issues the MMAs;
+// eight warps drain the accumulators.  CTA pairs (cta_group::2) work on 256 features x 256 channels: each CTA widens 128
+// features and stages 128 channels, so a widened element meets 256 channels.
+//
+// What bounds it: 4096 x 4096 over 8192 tokens takes 236 us (1.16 PFLOP/s; the same kernel without the widening's work 191).  A stage's
+// MMAs need 512 cycles, its traffic through shared memory (operands 32 KB, TMA 24 KB, widening 24 KB) 640 at 128 bytes a cycle, and the
+// widening warps' chains of dependent instructions add their latency.  The warps that wait cost little (naps between their
+// looks at a barrier changed nothing), and so does the depth of the rings (5 widened tiles and 5 stages: 242 us).
 //
 // Both operands are MN-major 16-bit tiles (a row of 128 bytes = 64 features or channels of one token, 128-byte swizzle,
 // repeating unit 8 tokens: SBO = 1024; chunks of 64 features I8W_BK * 128 bytes apart: LBO); one MMA takes 16 tokens = 2048 bytes.
@@ -321,8 +324,8 @@ i8_wgrad(const __grid_constant__ I8WgradArgs a, const __grid_constant__ I8Tensor
     } else if (warp >= 12) {
         // ---- widening: thread t of 256 takes features 16 (t % 8) .. + 15 of tokens t / 8 and t / 8 + 32 (the two chunks of 64
         // features of a token in swapped pairs: the eight lanes of a token pair's row then hit eight different units of the swizzled
-        // rows they write).  Four warps per scheduler with two vectors each: 4096 x 4096 over 8192 tokens takes 248 us, with half the
-        // warps and twice the vectors 262, with twelve warps away from the MMA issuer's scheduler 276
+        // rows they write).  Four warps per scheduler with two vectors each: with half the warps and twice the vectors 4096 x 4096
+        // over 8192 tokens took 262 us instead of 248, with twelve warps away from the MMA issuer's scheduler 249 instead of 236
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(I8W_REGS_WIDEN));
         const uint32_t group = (warp - 12) >> 3, t = (threadIdx.x - 384) & 255u, unit = t & 7u, chunk = unit >> 2, tok = (t >> 3) ^ chunk;
         const uint32_t ready_base = i8_map_to_cta(bar_ready, leader);
