@@ -173,6 +173,7 @@ def _ptr(x) -> int:
 
 
 _TYPE_CODES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3}
+_VECTORS = {"w_scale", "x_scale", "scale", "bias", "gamma"}
 _type_codes: dict = {}   # dtype object -> code, filled as dtypes are met
 
 
@@ -185,10 +186,12 @@ def _dtype_code(dtype) -> int:
 
 
 def _type_code(x, given: Optional[int]) -> int:
-    """Element type of a matrix: the one given, else the tensor's or array's own (FP32, FP16 or BF16)."""
-    if given is not None:
-        return int(given)
+    """Element type of a matrix: the one given, which must be a tensor's own where that is one of FP32, FP16 and BF16, else the tensor's."""
     code = _dtype_code(getattr(x, "dtype", None))
+    if given is not None:
+        if 0 <= code <= 2 and code != int(given):
+            raise TypeError(f"a tensor of {x.dtype} with the element type {given}")
+        return int(given)
     if not 0 <= code <= 2:
         raise TypeError(f"element type of {type(x).__name__} {getattr(x, 'dtype', '')}: pass a FP32, FP16 or BF16 tensor, or the "
                         f"type with an address")
@@ -266,16 +269,31 @@ class SgemmRunner:
 
     # ------------------------------------------------- 8-bit operands (cubins generated for INT8)
     def _addr(self, x, name: str, code: int = -1) -> int:
-        """Address of an operand of an 8-bit call; a tensor must lie on the handle's GPU, have the element type the
-        call takes (`code`, -1: any), and hold the elements of a row one after the other."""
-        if not hasattr(x, "data_ptr"):
+        """Address of an operand of an 8-bit call.  A tensor must lie on the handle's GPU, have the element type the call takes
+        (`code`, -1: any) and lie as the call reads it: a vector without gaps, a matrix with the elements of a row one after
+        the other and, where it has more than two dimensions, its rows at one distance throughout."""
+        if x is None or isinstance(x, int):
             return _ptr(x)
+        if not hasattr(x, "data_ptr"):
+            raise TypeError(f"{name} is a {type(x).__name__}: the call takes tensors on the handle's GPU or device addresses")
         if x.get_device() != self.device:
             raise ValueError(f"{name} lies on {x.device}, the handle on GPU {self.device}")
         if code >= 0 and _dtype_code(x.dtype) != code:
             raise TypeError(f"{name} is {x.dtype}, the call takes {[k for k, v in _TYPE_CODES.items() if v == code][0]}")
-        if not x.is_contiguous() and x.shape[-1] > 1 and x.stride(-1) != 1:
-            raise ValueError(f"{name}: the elements of a row must be contiguous")
+        if not x.is_contiguous():
+            if name in _VECTORS:
+                raise ValueError(f"{name}: the elements must be contiguous")
+            if x.shape[-1] > 1 and x.stride(-1) != 1:
+                raise ValueError(f"{name}: the elements of a row must be contiguous")
+            shape, stride = x.shape, x.stride()
+            rows = x.dim() - 2      # the dimension of the rows; a dimension of one has no distance of its own
+            for d in range(x.dim() - 3, -1, -1):
+                if shape[d] == 1:
+                    continue
+                # (one row per group: the pitch that the call would take is not the distance to the next group)
+                if shape[rows] == 1 or stride[d] != stride[rows] * shape[rows]:
+                    raise ValueError(f"{name}: its rows do not lie at one distance; pass one part at a time or a copy")
+                rows = d
         return x.data_ptr()
 
     # Operands are tensors on the handle's GPU or addresses (their element type then goes with ..._type: 0 FP32, 1 FP16, 2 BF16).  A leading
