@@ -89,7 +89,9 @@ struct Call {
         }
         return (uint32_t)v;
     }
-    // A leading dimension.  0: the row pitch of a tensor of two or more dimensions, else the columns lie one behind the other.
+    // A leading dimension.  0: the distance of the rows of a tensor of two or more dimensions, else the columns lie one behind the other.
+    // The rows' distance is that of the last dimension before the elements' that is longer than one: the stride of a dimension of
+    // one says nothing (a contiguous (rows, 1, elements) may carry any there).
     uint32_t ld(PyObject *given, PyObject *matrix, uint32_t rows) {
         const uint32_t v = u32(given), dense = rows ? rows : 1u;
         if (!ok || v || matrix == Py_None || PyLong_CheckExact(matrix)) return v ? v : dense;
@@ -100,9 +102,13 @@ struct Call {
         }
         uint32_t pitch = dense;
         if (PyTuple_Check(r) && PyTuple_GET_SIZE(r) >= 2) {
-            const long long stride = PyLong_AsLongLong(PyTuple_GET_ITEM(r, PyTuple_GET_SIZE(r) - 2));
+            const Py_ssize_t last = PyTuple_GET_SIZE(r) - 2;
+            long long stride = PyLong_AsLongLong(PyTuple_GET_ITEM(r, last));
+            const bool fits = stride >= (long long)dense && stride <= 0xFFFFFFFFll;
+            const Py_ssize_t dim = last > 0 || !fits ? row_dimension(matrix, last) : last;
+            if (dim >= 0) stride = PyLong_AsLongLong(PyTuple_GET_ITEM(r, dim));
             if (stride >= (long long)dense && stride <= 0xFFFFFFFFll) pitch = (uint32_t)stride;
-            else if (one_row(matrix)) pitch = dense;   // (the stride of a dimension of one says nothing)
+            else if (dim < 0) pitch = dense;
             else {
                 PyErr_Format(PyExc_ValueError, "a tensor's rows are %lld elements apart, the call reads %u of each", stride, dense);
                 ok = false;
@@ -111,17 +117,15 @@ struct Call {
         Py_DECREF(r);
         return pitch;
     }
-    bool one_row(PyObject *matrix) {
+    // the last dimension up to `last` that is longer than one, -1 if there is none
+    Py_ssize_t row_dimension(PyObject *matrix, Py_ssize_t last) {
         PyObject *shape = PyObject_GetAttr(matrix, s_shape);
-        bool one = false;
-        if (shape && PySequence_Check(shape) && PySequence_Size(shape) >= 2) {
-            PyObject *rows = PySequence_GetItem(shape, PySequence_Size(shape) - 2);
-            one = rows && PyLong_AsLong(rows) <= 1;
-            Py_XDECREF(rows);
-        }
+        Py_ssize_t d = last;
+        if (shape && PyTuple_Check(shape) && PyTuple_GET_SIZE(shape) > last)
+            while (d >= 0 && PyLong_AsLong(PyTuple_GET_ITEM(shape, d)) <= 1) --d;
         Py_XDECREF(shape);
         PyErr_Clear();
-        return one;
+        return d;
     }
     float f32(PyObject *x) {
         if (!ok) return 0.0f;
@@ -223,6 +227,19 @@ NATIVE_BEGIN(i8_wgrad, 17)
     void *stream = c.ptr(a[16]);
 NATIVE_END(sgemm_i8_wgrad(h, q, s, dy, dy_type, prior, dw, dw_type, alpha, beta, m, channels, tokens, ldq, lddy, ldc, lddw, stream))
 
+// pitch(matrix, row length): the leading dimension that the calls above take for a matrix
+PyObject *pitch(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    if (n != 2) {
+        PyErr_SetString(PyExc_TypeError, "pitch(matrix, row length)");
+        return nullptr;
+    }
+    Call c{nullptr, -1};
+    PyObject *zero = PyLong_FromLong(0);
+    const uint32_t rows = c.u32(v[1]), ld = zero ? c.ld(zero, v[0], rows) : 0;
+    Py_XDECREF(zero);
+    return c.ok && zero ? PyLong_FromUnsignedLong(ld) : nullptr;
+}
+
 // setup(type codes by dtype, api._type_code)
 PyObject *setup(PyObject *, PyObject *const *v, Py_ssize_t n) {
     if (n != 2 || !PyDict_Check(v[0]) || !PyCallable_Check(v[1])) {
@@ -239,7 +256,7 @@ PyObject *setup(PyObject *, PyObject *const *v, Py_ssize_t n) {
 #define NATIVE_METHOD(NAME) {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(NAME)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {
     NATIVE_METHOD(i8_linear), NATIVE_METHOD(i8_quantize), NATIVE_METHOD(i8_restore), NATIVE_METHOD(i8_rmsnorm), NATIVE_METHOD(i8_wgrad),
-    NATIVE_METHOD(setup), {nullptr, nullptr, 0, nullptr}};
+    NATIVE_METHOD(pitch), NATIVE_METHOD(setup), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_sgemm_native", "8-bit calls of runner.api without ctypes", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

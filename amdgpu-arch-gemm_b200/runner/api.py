@@ -285,19 +285,14 @@ class SgemmRunner:
                 raise ValueError(f"{name}: the elements must be contiguous")
             if x.shape[-1] > 1 and x.stride(-1) != 1:
                 raise ValueError(f"{name}: the elements of a row must be contiguous")
-            shape, stride = x.shape, x.stride()
-            rows = x.dim() - 2      # the dimension of the rows; a dimension of one has no distance of its own
-            for d in range(x.dim() - 3, -1, -1):
-                if shape[d] == 1:
-                    continue
-                # (one row per group: the pitch that the call would take is not the distance to the next group)
-                if shape[rows] == 1 or stride[d] != stride[rows] * shape[rows]:
-                    raise ValueError(f"{name}: its rows do not lie at one distance; pass one part at a time or a copy")
-                rows = d
+            # dimensions of one have no distance of their own; the others, from the rows outwards, must follow one another
+            outer = [(n, d) for n, d in zip(x.shape[:-1], x.stride()[:-1]) if n > 1]
+            if any(far != near * count for (_, far), (count, near) in zip(outer, outer[1:])):
+                raise ValueError(f"{name}: its rows do not lie at one distance; pass one part at a time or a copy")
         return x.data_ptr()
 
     # Operands are tensors on the handle's GPU or addresses (their element type then goes with ..._type: 0 FP32, 1 FP16, 2 BF16).  A leading
-    # dimension of 0 is the row pitch of a two-dimensional tensor, and for addresses the length of a row.
+    # dimension of 0 is the distance of a tensor's rows (of all its dimensions but the last), and for addresses the length of a row.
     def _i8(self, name: str, *args):
         if not self._h:
             raise SgemmError(-1, "sgemm_" + name, "the handle is closed")

@@ -158,10 +158,10 @@ def test_vectors_with_gaps_are_refused(name):
 def test_rows_at_uneven_distances_are_refused():
     r = bare_runner()
     base = torch.zeros(3, 6, 16)
-    for x in (base[:, :4], base[:, :4, :8], base[:, :1], base[::2], base.transpose(0, 1), torch.zeros(6, 16).expand(3, 6, 16)):
+    for x in (base[:, :4], base[:, :4, :8], base[::2], base.transpose(0, 1), torch.zeros(6, 16).expand(3, 6, 16)):
         with pytest.raises(ValueError, match="one distance"):
             r._addr(x, "x")
-    for x in (base, base[..., :8], base[:1, :4], base[1:2, 2:5, :3], base[:, :, :8][1], torch.zeros(2, 3, 6, 16)[..., :8]):
+    for x in (base, base[..., :8], base[:1, :4], base[1:2, 2:5, :3], base[:, :1], base[:, :, :8][1], torch.zeros(2, 3, 6, 16)[..., :8]):
         assert r._addr(x, "x") == x.data_ptr()
     with pytest.raises(ValueError, match="one distance"):
         r._addr(torch.zeros(2, 3, 6, 16)[:, :2], "x")
@@ -182,3 +182,21 @@ def test_a_type_that_is_not_the_tensors_is_refused(built):
     # its own type, and storage of another kind with the type said: only the NULL handle stops these
     assert api._native().i8_restore(bare_runner(), 0, -1, 1 << 20, 1 << 20, bf16, 8, 4, 0, 0, 2, 0) == -1
     assert api._native().i8_restore(bare_runner(), 0, -1, 1 << 20, 1 << 20, torch.zeros(4, 16, dtype=torch.uint8), 8, 4, 0, 0, 2, 0) == -1
+
+
+@pytest.mark.parametrize("shape, stride, rows, pitch", [
+    ((4, 8), (8, 1), 8, 8), ((4, 8), (24, 1), 8, 24), ((1, 8), (3, 1), 8, 8), ((1, 8), (32, 1), 8, 32), ((2, 3, 8), (36, 12, 1), 8, 12),
+    ((5, 1, 8), (8, 40, 1), 8, 8), ((5, 1, 8), (8, 1, 1), 8, 8), ((5, 1, 1, 8), (16, 9, 77, 1), 8, 16), ((1, 1, 8), (99, 16, 1), 8, 16),
+    ((8,), (1,), 8, 8), ((4, 8), (0, 1), 8, None), ((5, 1, 8), (4, 40, 1), 8, None)])
+def test_pitch_is_that_of_the_rows(built, shape, stride, rows, pitch):
+    x = torch.empty(4096, dtype=torch.int8).as_strided(shape, stride)
+    if pitch is None:
+        with pytest.raises(ValueError, match="elements apart"):
+            api._native().pitch(x, rows)
+    else:
+        assert api._native().pitch(x, rows) == pitch
+
+
+def test_pitch_of_a_transposed_batch_of_one(built):
+    x = torch.zeros(1, 5, 16, dtype=torch.int8).transpose(0, 1)
+    assert x.is_contiguous() and x.stride(-2) == 80 and api._native().pitch(x, 16) == 16
