@@ -30,6 +30,9 @@
 #define I8_ROUND_MAGIC 12582912.0f          // 1.5 * 2^23: adding it rounds to the nearest integer, into the low mantissa bits
 #define I8_LARGEST_BITS 0x7F7E0000u         // 127 * 2^121 as an FP32 word
 #define I8_TINY 0x1p-100f                   // peaks below it: 127 / P is not formed in FP32
+// Rows whose squares leave FP32 have a second sum, of (h * 2^-96)^2.  Of the largest FP32 number that is below 2^64, so the longest row's
+// (2^30) stays below 2^94; and where the plain sum passed 2^128, squares that matter to 2^-24 of it were above 2^74, here 2^-118.
+#define I8_DOWN 0x1p-96f
 
 struct I8RowArgs {
     const void *x;
@@ -189,11 +192,16 @@ __device__ __forceinline__ I8Rounding i8_rounding(uint32_t peak_bits, bool pow2,
     return r;
 }
 
-// rsqrt(mean + eps): the product with 1 / K is off by 2^-23 and rsqrtf by 2 of its last places
+// The norm's scale, `base` = P / 127 times rsqrt(mean + eps): the product with 1 / K is off by 2^-23 and rsqrtf by 2 of its last places
 template <uint32_t TYPE>
-__device__ __forceinline__ float i8_rstd(const float (&sums)[2], float inv_k, float eps) {
-    if (TYPE != SGEMM_I8_FP16 && !(sums[0] < INFINITY)) return 0x1p-64f * rsqrtf(sums[1] * inv_k);
-    return rsqrtf(fmaf(sums[0], inv_k, eps));
+__device__ __forceinline__ float i8_norm_scale(float base, const float (&sums)[2], float inv_k, float eps) {
+    const float mean = fmaf(sums[0], inv_k, eps);
+    if (TYPE != SGEMM_I8_FP16 && !(mean < INFINITY)) {   // (squares of FP16 sums cannot leave FP32)
+        // in 64 bits, where neither factor nor the product can leave the range: the root is between 2^-32 and 2^48 here
+        const float root = rsqrtf(fmaf(sums[1], inv_k, eps * I8_DOWN * I8_DOWN));
+        return (float)((double)base * (double)root * (double)I8_DOWN);
+    }
+    return base * rsqrtf(mean);
 }
 
 // The row's peak over its `tpr` threads (and its sums, in a fixed order).
@@ -258,7 +266,7 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
     };
     uint4 raw[NV];
     float p[NORM ? PER : 1];
-    float sums[2] = {0.0f, 0.0f};    // of h^2, and of (h * 2^-64)^2 for rows whose squares leave FP32
+    float sums[2] = {0.0f, 0.0f};    // of h^2, and of (h * 2^-96)^2 for rows whose squares leave FP32
     uint32_t peak_pair = 0u;
     float peak = 0.0f;
     auto fetch = [&](uint32_t pass, bool store_sum) {
@@ -284,12 +292,12 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
             float squares = 0.0f;
 #pragma unroll
             for (int j = 0; j < PER; ++j) squares = fmaf(p[j], p[j], squares);
-            float small = squares * 0x1p-64f * 0x1p-64f;
+            float small = squares * I8_DOWN * I8_DOWN;
             if (TYPE != SGEMM_I8_FP16 && !(squares < INFINITY)) {   // (squares of FP16 sums cannot leave FP32)
                 small = 0.0f;
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    const float v = p[j] * 0x1p-64f;
+                    const float v = p[j] * I8_DOWN;
                     small = fmaf(v, v, small);
                 }
             }
@@ -346,8 +354,7 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
     if (!live) return;   // (a warp has one row: tpr is at least 32)
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (NORM) scale *= i8_rstd<TYPE>(sums, a.inv_k, a.eps);
-    if (t == 0) a.scale[row] = scale;
+    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.inv_k, a.eps) : scale;
 
     for (uint32_t pass = 0; pass < passes; ++pass) {
         if (passes > 1) fetch(pass, true);
@@ -446,7 +453,7 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
             for (int j = 0; j < PER; ++j) {
                 sums[0] = fmaf(p[j], p[j], sums[0]);
                 if (TYPE != SGEMM_I8_FP16) {
-                    const float small = p[j] * 0x1p-64f;
+                    const float small = p[j] * I8_DOWN;
                     sums[1] = fmaf(small, small, sums[1]);
                 }
                 p[j] = __fmul_rn(p[j], first + j * a.tpr < k ? E::get(__ldg(g + first + j * a.tpr)) : 0.0f);
@@ -462,8 +469,7 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
     if (!live) return;
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (NORM) scale *= i8_rstd<TYPE>(sums, a.inv_k, a.eps);
-    if (t == 0) a.scale[row] = scale;
+    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.inv_k, a.eps) : scale;
     for (uint32_t pass = 0; pass < passes; ++pass) {
         if (passes > 1) fetch(pass, true);
         const uint32_t first = pass * span + t;
