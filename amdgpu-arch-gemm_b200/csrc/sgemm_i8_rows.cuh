@@ -33,6 +33,10 @@
 // Rows whose squares leave FP32 have a second sum, of (h * 2^-96)^2.  Of the largest FP32 number that is below 2^64, so the longest row's
 // (2^30) stays below 2^94; and where the plain sum passed 2^128, squares that matter to 2^-24 of it were above 2^74, here 2^-118.
 #define I8_DOWN 0x1p-96f
+// Where neither the plain sum nor eps reaches 2^-90, squares may vanish: a third sum, of (h * 2^92)^2, stays below 2^94 there, and the square of
+// the smallest FP32 number is 2^-114 in it.  (A plain sum of at least 2^-90 lacks at most 2^30 * 2^-150.)
+#define I8_FAINT 0x1p-90f
+#define I8_UP 0x1p92f
 
 struct I8RowArgs {
     const void *x;
@@ -192,10 +196,16 @@ __device__ __forceinline__ I8Rounding i8_rounding(uint32_t peak_bits, bool pow2,
     return r;
 }
 
-// The norm's scale, `base` = P / 127 times rsqrt(mean + eps): the product with 1 / K is off by 2^-23 and rsqrtf by 2 of its last places
+// The norm's scale, `base` = P / 127 times rsqrt(mean + eps), 0 for a row whose P is 0: the product with 1 / K is off by 2^-23 and rsqrtf by 2
+// of its last places
 template <uint32_t TYPE>
-__device__ __forceinline__ float i8_norm_scale(float base, const float (&sums)[2], float inv_k, float eps) {
+__device__ __forceinline__ float i8_norm_scale(float base, const float (&sums)[3], uint32_t k, float inv_k, float eps) {
     const float mean = fmaf(sums[0], inv_k, eps);
+    if (base == 0.0f) return 0.0f;
+    if (TYPE != SGEMM_I8_FP16 && eps < I8_FAINT && sums[0] < I8_FAINT) {   // (squares of FP16 numbers are at least 2^-48)
+        const float n = (float)k, root = rsqrtf(fmaf(eps * I8_UP * I8_UP, n, sums[2])) * sqrtf(n);   // (1 / K could make the mean vanish again)
+        return (float)((double)base * (double)root * (double)I8_UP);
+    }
     if (TYPE != SGEMM_I8_FP16 && !(mean < INFINITY)) {   // (squares of FP16 sums cannot leave FP32)
         // in 64 bits, where neither factor nor the product can leave the range: the root is between 2^-32 and 2^48 here
         const float root = rsqrtf(fmaf(sums[1], inv_k, eps * I8_DOWN * I8_DOWN));
@@ -204,16 +214,18 @@ __device__ __forceinline__ float i8_norm_scale(float base, const float (&sums)[2
     return base * rsqrtf(mean);
 }
 
-// The row's peak over its `tpr` threads (and its sums, in a fixed order).
+// The row's peak over its `tpr` threads (and its first `count` sums, at most SUMS, in a fixed order).
 template <int SUMS>
-__device__ __forceinline__ void i8_row_reduce(uint32_t &peak_bits, float (&sums)[2], uint32_t tpr) {
-    __shared__ float red_sum[2][32];
+__device__ __forceinline__ void i8_row_reduce(uint32_t &peak_bits, float (&sums)[3], int count, uint32_t tpr) {
+    __shared__ float red_sum[3][32];
     __shared__ uint32_t red_max[32];
     peak_bits = __reduce_max_sync(0xffffffffu, peak_bits);
 #pragma unroll
-    for (int i = 0; i < SUMS; ++i)
+    for (int i = 0; i < SUMS; ++i) {
+        if (i >= count) break;
 #pragma unroll
         for (int d = 16; d; d >>= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], d);
+    }
     if (tpr <= 32) return;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = tpr >> 5, first = warp & ~(warps - 1);
     if (lane == 0) {
@@ -226,6 +238,7 @@ __device__ __forceinline__ void i8_row_reduce(uint32_t &peak_bits, float (&sums)
     peak_bits = __reduce_max_sync(0xffffffffu, mine ? red_max[first + lane] : 0u);
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) {
+        if (i >= count) break;
         sums[i] = mine ? red_sum[i][first + lane] : 0.0f;
 #pragma unroll
         for (int d = 16; d; d >>= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], d);
@@ -266,7 +279,8 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
     };
     uint4 raw[NV];
     float p[NORM ? PER : 1];
-    float sums[2] = {0.0f, 0.0f};    // of h^2, and of (h * 2^-96)^2 for rows whose squares leave FP32
+    float sums[3] = {0.0f, 0.0f, 0.0f};    // of h^2, of (h * 2^-96)^2 for rows whose squares leave FP32, of (h * 2^92)^2 for those whose squares vanish
+    const bool faint = NORM && TYPE != SGEMM_I8_FP16 && a.eps < I8_FAINT;   // the third is taken
     uint32_t peak_pair = 0u;
     float peak = 0.0f;
     auto fetch = [&](uint32_t pass, bool store_sum) {
@@ -303,6 +317,15 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
             }
             sums[0] += squares;
             sums[1] += small;
+            if (faint) {
+                float large = 0.0f;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const float v = p[j] * I8_UP;
+                    large = fmaf(v, v, large);
+                }
+                sums[2] += large;
+            }
             if (sum && store_sum) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
@@ -350,11 +373,11 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
         peak = both[0];
     }
     uint32_t peak_bits = i8_abs_bits(peak);
-    i8_row_reduce<NORM ? (TYPE == SGEMM_I8_FP16 ? 1 : 2) : 0>(peak_bits, sums, a.tpr);
+    i8_row_reduce<NORM ? (TYPE == SGEMM_I8_FP16 ? 1 : 3) : 0>(peak_bits, sums, faint ? 3 : 2, a.tpr);
     if (!live) return;   // (a warp has one row: tpr is at least 32)
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.inv_k, a.eps) : scale;
+    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.k, a.inv_k, a.eps) : scale;
 
     for (uint32_t pass = 0; pass < passes; ++pass) {
         if (passes > 1) fetch(pass, true);
@@ -430,7 +453,8 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
     const uint32_t k = live ? a.k : 0u, span = a.tpr * PER;
     const uint32_t passes = a.passes;
     float p[PER];
-    float sums[2] = {0.0f, 0.0f};
+    float sums[3] = {0.0f, 0.0f, 0.0f};
+    const bool faint = NORM && TYPE != SGEMM_I8_FP16 && a.eps < I8_FAINT;
     uint32_t peak_bits = 0u;
     auto fetch = [&](uint32_t pass, bool store_sum) {
         const uint32_t first = pass * span + t;
@@ -455,6 +479,10 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
                 if (TYPE != SGEMM_I8_FP16) {
                     const float small = p[j] * I8_DOWN;
                     sums[1] = fmaf(small, small, sums[1]);
+                    if (faint) {
+                        const float large = p[j] * I8_UP;
+                        sums[2] = fmaf(large, large, sums[2]);
+                    }
                 }
                 p[j] = __fmul_rn(p[j], first + j * a.tpr < k ? E::get(__ldg(g + first + j * a.tpr)) : 0.0f);
             }
@@ -465,11 +493,11 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) peak_bits = max(peak_bits, i8_abs_bits(p[j]));
     }
-    i8_row_reduce<NORM ? (TYPE == SGEMM_I8_FP16 ? 1 : 2) : 0>(peak_bits, sums, a.tpr);
+    i8_row_reduce<NORM ? (TYPE == SGEMM_I8_FP16 ? 1 : 3) : 0>(peak_bits, sums, faint ? 3 : 2, a.tpr);
     if (!live) return;
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.inv_k, a.eps) : scale;
+    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.k, a.inv_k, a.eps) : scale;
     for (uint32_t pass = 0; pass < passes; ++pass) {
         if (passes > 1) fetch(pass, true);
         const uint32_t first = pass * span + t;

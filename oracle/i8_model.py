@@ -62,9 +62,9 @@ def rmsnorm(x, gamma, eps, residual=None):
         p = (h * np.asarray(gamma, dtype=f32)[None, :]).astype(np.float64)
     q, base = quantize(p)
     wide = h.astype(np.float64)
-    with np.errstate(over="ignore", invalid="ignore"):
+    with np.errstate(over="ignore", invalid="ignore", divide="ignore"):
         rstd = 1.0 / np.sqrt(np.mean(wide * wide, axis=1) + eps)
-    return q, base * rstd, wide
+        return q, np.where(base == 0, 0.0, base * rstd), wide
 
 
 def restore(q, scale, kind):

@@ -70,3 +70,45 @@ def test_a_full_prompt_of_large_rows(r, kind):   # noqa: F811
     assert (np.abs(got[0]) == 127).all()
     check_rounded(got[1], np.full(2000, 1.0 / 127.0), "fp32", 66 * 2.0 ** -24)
     assert np.array_equal(got[2], model.round_to(x, kind))
+
+
+# Rows whose squares vanish in FP32: exponents of their magnitudes.
+SMALL = {"fp32": [0, -30, -44, -46, -60, -63, -70, -75, -80, -100], "bf16": [0, -30, -44, -46, -60, -63, -70, -75, -80, -100], "fp16": [0, -10, -14, -20, -22]}
+EPS = [0.0, 2.0 ** -149, 2.0 ** -130, 2.0 ** -91, 2.0 ** -89, 1e-20, 1e-6]
+
+
+def small_rows(k, kind, sizes):
+    """Rows of zeros, of the given magnitudes, and (the third) one of a single number among zeros."""
+    rng = np.random.default_rng(k)
+    x = rounded(rng.choice([-1, 1], (len(sizes) + 1, k)) * rng.uniform(0.5, 0.99, (len(sizes) + 1, k)) * 2.0 ** np.array([0] + sizes)[:, None], kind)
+    x[0] = 0.0
+    x[2, 1:] = 0.0
+    return x, rounded(rng.uniform(0.5, 1.0, k), kind)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("k", [1, 300, 4096, 40000])
+@pytest.mark.parametrize("eps", EPS)
+def test_small_rows_and_small_eps(r, kind, form, k, eps):   # noqa: F811
+    """A row of zeros has scale 0 for every eps, one that is not has the definition's scale.  (Squares below the normal
+    numbers are summed again from values times 2^92.  The root of K in place of 1 / K, one more product: within the bound, which had
+    6 * 2^-24 to spare.)"""
+    x, gamma = small_rows(k, kind, SMALL[kind])
+    eps = float(np.float32(eps))
+    for power in (0, -10):
+        g = rounded(gamma * 2.0 ** power, kind)
+        got = call(r, x, g, kind, eps, form)
+        check_norm(got, x, g, kind, np.zeros_like(x), eps=eps, passes=1 + k // 8192)
+        assert got[1][0] == 0 and (got[0][0] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+def test_a_padding_row_of_zeros_without_eps(r, kind):   # noqa: F811
+    rng = np.random.default_rng(2)
+    x = rounded(rng.standard_normal((12, 300)), kind)
+    x[4] = 0.0
+    g = rounded(rng.standard_normal(300), kind)
+    got = rmsnorm(r, x, g, kind, eps=0.0, want_sum=False)
+    check_norm(got, x, g, kind, eps=0.0)
+    assert got[1][4] == 0 and (got[0][4] == 0).all()
