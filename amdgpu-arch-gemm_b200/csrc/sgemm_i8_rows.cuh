@@ -196,22 +196,36 @@ __device__ __forceinline__ I8Rounding i8_rounding(uint32_t peak_bits, bool pow2,
     return r;
 }
 
-// The norm's scale, `base` = P / 127 times rsqrt(mean + eps), 0 for a row whose P is 0: the product with 1 / K is off by 2^-23 and rsqrtf by 2
-// of its last places
+// The norm's scale outside of the ordinary range (out of line: a row in thousands, and its 64-bit code would lie in everybody's way).  The root
+// comes from the sum that is in range, P / 127, which has few bits left below the normal numbers, is formed from P * 2^100, and the
+// powers of two come off in 64 bits, where nothing on the way can leave the range.
+__device__ __noinline__ float i8_norm_scale_far(float peak, float plain, float down, float up, uint32_t k, float inv_k, float eps) {
+    if (peak == 0.0f) return 0.0f;
+    const float mean = fmaf(plain, inv_k, eps);
+    float root;
+    double factor = 1.0;
+    if (eps < I8_FAINT && plain < I8_FAINT) {
+        const float n = (float)k;   // (1 / K could make the mean vanish again)
+        root = rsqrtf(fmaf(eps * I8_UP * I8_UP, n, up)) * sqrtf(n);
+        factor = (double)I8_UP;
+    } else if (!(mean < INFINITY)) {
+        root = rsqrtf(fmaf(down, inv_k, eps * I8_DOWN * I8_DOWN));
+        factor = (double)I8_DOWN;
+    } else {
+        root = rsqrtf(mean);
+    }
+    const bool tiny = peak < I8_TINY;
+    const float base = __fdiv_rn(tiny ? peak * 0x1p100f : peak, 127.0f);
+    return (float)((double)base * (double)root * (tiny ? factor * 0x1p-100 : factor));
+}
+// The norm's scale, `base` = P / 127 (NaN where P is out of range) times rsqrt(mean + eps), 0 for a row whose P is 0: the product with 1 / K is off
+// by 2^-23 and rsqrtf by 2 of its last places.
 template <uint32_t TYPE>
-__device__ __forceinline__ float i8_norm_scale(float base, const float (&sums)[3], uint32_t k, float inv_k, float eps) {
+__device__ __forceinline__ float i8_norm_scale(float peak, float base, const float (&sums)[3], uint32_t k, float inv_k, float eps) {
     const float mean = fmaf(sums[0], inv_k, eps);
-    if (base == 0.0f) return 0.0f;
-    if (TYPE != SGEMM_I8_FP16 && eps < I8_FAINT && sums[0] < I8_FAINT) {   // (squares of FP16 numbers are at least 2^-48)
-        const float n = (float)k, root = rsqrtf(fmaf(eps * I8_UP * I8_UP, n, sums[2])) * sqrtf(n);   // (1 / K could make the mean vanish again)
-        return (float)((double)base * (double)root * (double)I8_UP);
-    }
-    if (TYPE != SGEMM_I8_FP16 && !(mean < INFINITY)) {   // (squares of FP16 sums cannot leave FP32)
-        // in 64 bits, where neither factor nor the product can leave the range: the root is between 2^-32 and 2^48 here
-        const float root = rsqrtf(fmaf(sums[1], inv_k, eps * I8_DOWN * I8_DOWN));
-        return (float)((double)base * (double)root * (double)I8_DOWN);
-    }
-    return base * rsqrtf(mean);
+    if (TYPE == SGEMM_I8_FP16) return peak == 0.0f ? 0.0f : base * rsqrtf(mean);   // squares and products are at least 2^-48, sums stay in range
+    if (isnan(base) || (peak >= I8_TINY && mean < INFINITY && (eps >= I8_FAINT || sums[0] >= I8_FAINT))) return base * rsqrtf(mean);
+    return i8_norm_scale_far(peak, sums[0], sums[1], sums[2], k, inv_k, eps);
 }
 
 // The row's peak over its `tpr` threads (and its first `count` sums, at most SUMS, in a fixed order).
@@ -377,7 +391,7 @@ __device__ __forceinline__ void i8_rows_vector(const I8RowArgs &a) {
     if (!live) return;   // (a warp has one row: tpr is at least 32)
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.k, a.inv_k, a.eps) : scale;
+    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(rounding.peak, scale, sums, a.k, a.inv_k, a.eps) : scale;
 
     for (uint32_t pass = 0; pass < passes; ++pass) {
         if (passes > 1) fetch(pass, true);
@@ -497,7 +511,7 @@ __device__ __forceinline__ void i8_rows_scalar(const I8RowArgs &a) {
     if (!live) return;
     float scale;
     const I8Rounding rounding = i8_rounding(peak_bits, !NORM && a.pow2 != 0u, scale);
-    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(scale, sums, a.k, a.inv_k, a.eps) : scale;
+    if (t == 0) a.scale[row] = NORM ? i8_norm_scale<TYPE>(rounding.peak, scale, sums, a.k, a.inv_k, a.eps) : scale;
     for (uint32_t pass = 0; pass < passes; ++pass) {
         if (passes > 1) fetch(pass, true);
         const uint32_t first = pass * span + t;

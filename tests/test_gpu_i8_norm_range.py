@@ -112,3 +112,18 @@ def test_a_padding_row_of_zeros_without_eps(r, kind):   # noqa: F811
     got = rmsnorm(r, x, g, kind, eps=0.0, want_sum=False)
     check_norm(got, x, g, kind, eps=0.0)
     assert got[1][4] == 0 and (got[0][4] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("k", [1, 300, 4096, 40000])
+@pytest.mark.parametrize("eps", EPS)
+def test_peaks_whose_127th_is_below_the_normal_numbers(r, kind, form, k, eps):   # noqa: F811
+    """Small rows, small gamma or both: the scale is one rounding away from the definition however small max |h * gamma| / 127 is."""
+    x, gamma = small_rows(k, kind, [0, -10, -100, -110, -120, -126, -131] + [-140, -147] * (kind == "fp32"))
+    eps = float(np.float32(eps))
+    for power in (0, -30, -110, -120):
+        g = rounded(gamma * 2.0 ** power, kind)
+        got = call(r, x, g, kind, eps, form)
+        check_norm(got, x, g, kind, np.zeros_like(x), eps=eps, passes=1 + k // 8192)
+        assert got[1][0] == 0 and (got[0][0] == 0).all()
