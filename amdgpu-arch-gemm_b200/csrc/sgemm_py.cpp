@@ -146,7 +146,8 @@ struct Call {
     }
 };
 
-// Every function: (runner, handle, device, arguments in the order of the SgemmRunner method) -> status of the C call.
+// Every function: (runner, handle, device, arguments in the order of the SgemmRunner method) -> status of the C call.  The C call runs without the
+// interpreter's lock, as calls through ctypes do: a launch can wait for room in the queue, and the stream for another Python thread.
 #define NATIVE_BEGIN(NAME, COUNT)                                                                        \
     PyObject *NAME(PyObject *, PyObject *const *v, Py_ssize_t n) {                                       \
         if (n != 3 + (COUNT)) {                                                                          \
@@ -158,7 +159,10 @@ struct Call {
         PyObject *const *a = v + 3;
 #define NATIVE_END(CALL)                  \
         if (!c.ok) return nullptr;        \
-        const int rc = (CALL);            \
+        int rc;                           \
+        Py_BEGIN_ALLOW_THREADS            \
+        rc = (CALL);                      \
+        Py_END_ALLOW_THREADS              \
         return PyLong_FromLong(rc);       \
     }
 
