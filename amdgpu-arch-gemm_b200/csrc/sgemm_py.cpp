@@ -80,6 +80,13 @@ struct Call {
         if (PyErr_Occurred()) ok = false;
         return (int)code;
     }
+    // address of an operand of the type that another one has: its own where none is given, and then this one must have it too; a given one
+    // holds for tensors of a known type, as it does for that other operand
+    void *sibling(PyObject *x, const char *name, int of, PyObject *given) {
+        if (given == Py_None) return addr(x, name, of);
+        if (ok && x != Py_None && !PyLong_CheckExact(x)) type(x, given);
+        return addr(x, name, -1);
+    }
     uint32_t u32(PyObject *x) {
         if (!ok) return 0;
         const unsigned long long v = PyLong_Check(x) ? PyLong_AsUnsignedLongLong(x) : PyNumber_AsSsize_t(x, PyExc_OverflowError);
@@ -205,13 +212,12 @@ NATIVE_END(sgemm_i8_restore(h, q, s, out, type, k, rows, ldq, ldo, stream))
 // x, gamma, q, scale, k, n, residual, sum_out, eps, ldx, ldr, ldq, lds, x_type, stream
 NATIVE_BEGIN(i8_rmsnorm, 15)
     const int type = c.type(a[0], a[13]);
-    const long same = a[13] == Py_None ? type : -1;
-    const void *x = c.addr(a[0], "x", -1), *g = c.addr(a[1], "gamma", same);
+    const void *x = c.addr(a[0], "x", -1), *g = c.sibling(a[1], "gamma", type, a[13]);
     auto *q = static_cast<int8_t *>(c.addr(a[2], "q", 3));
     auto *s = static_cast<float *>(c.addr(a[3], "scale", 0));
     const uint32_t k = c.u32(a[4]), rows = c.u32(a[5]);
-    const void *res = c.addr(a[6], "residual", same);
-    void *sum = c.addr(a[7], "sum_out", same);
+    const void *res = c.sibling(a[6], "residual", type, a[13]);
+    void *sum = c.sibling(a[7], "sum_out", type, a[13]);
     const float eps = c.f32(a[8]);
     const uint32_t ldx = c.ld(a[9], a[0], k), ldr = c.ld(a[10], a[6], k), ldq = c.ld(a[11], a[2], k), lds = c.ld(a[12], a[7], k);
     void *stream = c.ptr(a[14]);
@@ -225,7 +231,7 @@ NATIVE_BEGIN(i8_wgrad, 17)
     void *dw = c.addr(a[3], "dw", -1);
     const uint32_t m = c.u32(a[4]), channels = c.u32(a[5]), tokens = c.u32(a[6]);
     const int dy_type = c.type(a[2], a[14]), dw_type = c.type(a[3], a[15]);
-    const void *prior = c.addr(a[7], "c", a[15] == Py_None ? dw_type : -1);
+    const void *prior = c.sibling(a[7], "c", dw_type, a[15]);
     const float alpha = c.f32(a[8]), beta = c.f32(a[9]);
     const uint32_t ldq = c.ld(a[10], a[0], m), lddy = c.ld(a[11], a[2], channels), ldc = c.ld(a[12], a[7], m), lddw = c.ld(a[13], a[3], m);
     void *stream = c.ptr(a[16]);

@@ -74,3 +74,31 @@ def test_other_threads_run_while_a_call_waits(seam, r, name):
     finally:
         other.join()
         value(seam, "seam_wait", 0)
+
+
+def norm(seam, r, x=A, g=A, res=None, total=None, x_type=None):
+    return seam.i8_rmsnorm(r, 0, -1, x, g, A, A, 32, 4, res, total, 1e-6, 0, 0, 0, 0, x_type, 0)
+
+
+def test_a_given_type_holds_for_every_operand_of_that_type(seam, r):
+    """x_type beside tensors: gamma, the residual and the sum must have it, or be storage of another kind; so C and dw_type."""
+    f, h, raw = torch.zeros(4, 32), torch.zeros(4, 32, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.int16)
+    assert norm(seam, r, g=f[0], res=f, total=f, x_type=0) == 0 and norm(seam, r, h, h[0], h, h, x_type=2) == 0
+    assert norm(seam, r, raw, raw[0], raw, raw, x_type=2) == 0 and norm(seam, r, h, raw[0], raw, h, x_type=2) == 0
+    for code in (0, 1):
+        for bad in (dict(x=h), dict(g=h[0]), dict(res=h), dict(total=h)):
+            with pytest.raises(TypeError, match="element type"):
+                norm(seam, r, **bad, x_type=code)
+    for bad in (dict(g=h[0]), dict(res=h), dict(total=h)):       # without one: x's own
+        with pytest.raises(TypeError):
+            norm(seam, r, x=f, **bad)
+
+    def wgrad(c, dw=A, dw_type=None):
+        return seam.i8_wgrad(r, 0, -1, A, A, A, dw, 32, 4, 8, c, 1.0, 1.0, 0, 0, 0, 0, 2, dw_type, 0)
+
+    assert wgrad(h, dw_type=2) == 0 and wgrad(h, h) == 0 and wgrad(raw, h, 2) == 0
+    for code in (0, 1):
+        with pytest.raises(TypeError, match="element type"):
+            wgrad(h, dw_type=code)
+    with pytest.raises(TypeError):
+        wgrad(h, f)
