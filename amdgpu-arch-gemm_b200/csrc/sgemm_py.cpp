@@ -11,7 +11,7 @@
 
 namespace {
 
-PyObject *s_data_ptr, *s_get_device, *s_dtype, *s_is_contiguous, *s_addr, *s_stride, *s_shape;   // interned names
+PyObject *s_data_ptr, *s_get_device, *s_dtype, *s_is_contiguous, *s_addr, *s_stride, *s_shape, *s_element_size;   // interned names
 PyObject *g_codes = nullptr;       // dtype object -> type code (api._type_codes)
 PyObject *g_type_code = nullptr;   // api._type_code
 
@@ -98,8 +98,9 @@ struct Call {
     }
     // A leading dimension.  0: the distance of the rows of a tensor of two or more dimensions, else the columns lie one behind the other.
     // The rows' distance is that of the last dimension before the elements' that is longer than one: the stride of a dimension of
-    // one says nothing (a contiguous (rows, 1, elements) may carry any there).
-    uint32_t ld(PyObject *given, PyObject *matrix, uint32_t rows) {
+    // one says nothing (a contiguous (rows, 1, elements) may carry any there).  `type`: the element type where it was given in the call
+    // (else None): the tensor may then be storage of another kind, whose strides are in its own elements.
+    uint32_t ld(PyObject *given, PyObject *matrix, uint32_t rows, PyObject *type = Py_None, int code = -1) {
         const uint32_t v = u32(given), dense = rows ? rows : 1u;
         if (!ok || v || matrix == Py_None || PyLong_CheckExact(matrix)) return v ? v : dense;
         PyObject *r = PyObject_CallMethodNoArgs(matrix, s_stride);   // a tuple; an object without one is dense
@@ -110,14 +111,24 @@ struct Call {
         uint32_t pitch = dense;
         if (PyTuple_Check(r) && PyTuple_GET_SIZE(r) >= 2) {
             const Py_ssize_t last = PyTuple_GET_SIZE(r) - 2;
-            long long stride = PyLong_AsLongLong(PyTuple_GET_ITEM(r, last));
+            long long wide = 1, narrow = 1;   // bytes of the tensor's elements and of the call's
+            if (type != Py_None && code_of(matrix) != code) {
+                wide = element_size(matrix);
+                narrow = code == 0 ? 4 : 2;
+            }
+            const auto stride_of = [&](Py_ssize_t dim) -> long long {
+                const long long bytes = PyLong_AsLongLong(PyTuple_GET_ITEM(r, dim)) * wide;
+                return bytes % narrow ? -1 : bytes / narrow;
+            };
+            long long stride = stride_of(last);
             const bool fits = stride >= (long long)dense && stride <= 0xFFFFFFFFll;
             const Py_ssize_t dim = last > 0 || !fits ? row_dimension(matrix, last) : last;
-            if (dim >= 0) stride = PyLong_AsLongLong(PyTuple_GET_ITEM(r, dim));
+            if (dim >= 0) stride = stride_of(dim);
             if (stride >= (long long)dense && stride <= 0xFFFFFFFFll) pitch = (uint32_t)stride;
             else if (dim < 0) pitch = dense;
             else {
-                PyErr_Format(PyExc_ValueError, "a tensor's rows are %lld elements apart, the call reads %u of each", stride, dense);
+                if (stride < 0) PyErr_SetString(PyExc_ValueError, "a tensor's rows are no whole number of the given type's elements apart");
+                else PyErr_Format(PyExc_ValueError, "a tensor's rows are %lld elements apart, the call reads %u of each", stride, dense);
                 ok = false;
             }
         }
@@ -133,6 +144,13 @@ struct Call {
         Py_XDECREF(shape);
         PyErr_Clear();
         return d;
+    }
+    long long element_size(PyObject *x) {
+        PyObject *r = PyObject_CallMethodNoArgs(x, s_element_size);
+        const long long v = r ? PyLong_AsLongLong(r) : 1;
+        Py_XDECREF(r);
+        PyErr_Clear();   // (an object without one: in elements of the call's type)
+        return v > 0 ? v : 1;
     }
     float f32(PyObject *x) {
         if (!ok) return 0.0f;
@@ -182,8 +200,8 @@ NATIVE_BEGIN(i8_linear, 14)
     void *y = c.addr(a[4], "y", -1);
     const uint32_t m = c.u32(a[5]), tokens = c.u32(a[6]), k = c.u32(a[7]);
     const auto *bias = static_cast<const float *>(c.addr(a[8], "bias", 0));
-    const uint32_t ldw = c.ld(a[9], a[0], k), ldx = c.ld(a[10], a[2], k), ldy = c.ld(a[11], a[4], m);
     const int type = c.type(a[4], a[12]);
+    const uint32_t ldw = c.ld(a[9], a[0], k), ldx = c.ld(a[10], a[2], k), ldy = c.ld(a[11], a[4], m, a[12], type);
     void *stream = c.ptr(a[13]);
 NATIVE_END(sgemm_i8_linear(h, w, ws, x, xs, bias, y, type, m, tokens, k, ldw, ldx, ldy, stream))
 
@@ -194,8 +212,8 @@ NATIVE_BEGIN(i8_quantize, 10)
     auto *s = static_cast<float *>(c.addr(a[2], "scale", 0));
     const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]);
     const int pow2 = c.flag(a[5]);
-    const uint32_t ldx = c.ld(a[6], a[0], k), ldq = c.ld(a[7], a[1], k);
     const int type = c.type(a[0], a[8]);
+    const uint32_t ldx = c.ld(a[6], a[0], k, a[8], type), ldq = c.ld(a[7], a[1], k);
     void *stream = c.ptr(a[9]);
 NATIVE_END(sgemm_i8_quantize(h, x, type, q, s, k, rows, ldx, ldq, pow2, stream))
 
@@ -204,8 +222,9 @@ NATIVE_BEGIN(i8_restore, 9)
     const auto *q = static_cast<const int8_t *>(c.addr(a[0], "q", 3));
     const auto *s = static_cast<const float *>(c.addr(a[1], "scale", 0));
     void *out = c.addr(a[2], "out", -1);
-    const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]), ldq = c.ld(a[5], a[0], k), ldo = c.ld(a[6], a[2], k);
+    const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]);
     const int type = c.type(a[2], a[7]);
+    const uint32_t ldq = c.ld(a[5], a[0], k), ldo = c.ld(a[6], a[2], k, a[7], type);
     void *stream = c.ptr(a[8]);
 NATIVE_END(sgemm_i8_restore(h, q, s, out, type, k, rows, ldq, ldo, stream))
 
@@ -219,7 +238,8 @@ NATIVE_BEGIN(i8_rmsnorm, 15)
     const void *res = c.sibling(a[6], "residual", type, a[13]);
     void *sum = c.sibling(a[7], "sum_out", type, a[13]);
     const float eps = c.f32(a[8]);
-    const uint32_t ldx = c.ld(a[9], a[0], k), ldr = c.ld(a[10], a[6], k), ldq = c.ld(a[11], a[2], k), lds = c.ld(a[12], a[7], k);
+    const uint32_t ldx = c.ld(a[9], a[0], k, a[13], type), ldr = c.ld(a[10], a[6], k, a[13], type), ldq = c.ld(a[11], a[2], k),
+                   lds = c.ld(a[12], a[7], k, a[13], type);
     void *stream = c.ptr(a[14]);
 NATIVE_END(sgemm_i8_rmsnorm(h, x, res, g, type, eps, q, s, sum, k, rows, ldx, ldr, ldq, lds, stream))
 
@@ -233,7 +253,8 @@ NATIVE_BEGIN(i8_wgrad, 17)
     const int dy_type = c.type(a[2], a[14]), dw_type = c.type(a[3], a[15]);
     const void *prior = c.sibling(a[7], "c", dw_type, a[15]);
     const float alpha = c.f32(a[8]), beta = c.f32(a[9]);
-    const uint32_t ldq = c.ld(a[10], a[0], m), lddy = c.ld(a[11], a[2], channels), ldc = c.ld(a[12], a[7], m), lddw = c.ld(a[13], a[3], m);
+    const uint32_t ldq = c.ld(a[10], a[0], m), lddy = c.ld(a[11], a[2], channels, a[14], dy_type), ldc = c.ld(a[12], a[7], m, a[15], dw_type),
+                   lddw = c.ld(a[13], a[3], m, a[15], dw_type);
     void *stream = c.ptr(a[16]);
 NATIVE_END(sgemm_i8_wgrad(h, q, s, dy, dy_type, prior, dw, dw_type, alpha, beta, m, channels, tokens, ldq, lddy, ldc, lddw, stream))
 
@@ -279,6 +300,7 @@ PyMODINIT_FUNC PyInit__sgemm_native(void) {
     s_addr = PyUnicode_InternFromString("_addr");
     s_stride = PyUnicode_InternFromString("stride");
     s_shape = PyUnicode_InternFromString("shape");
-    if (!s_stride || !s_shape || !s_data_ptr || !s_get_device || !s_dtype || !s_is_contiguous || !s_addr) return nullptr;
+    s_element_size = PyUnicode_InternFromString("element_size");
+    if (!s_stride || !s_shape || !s_element_size || !s_data_ptr || !s_get_device || !s_dtype || !s_is_contiguous || !s_addr) return nullptr;
     return PyModule_Create(&g_module);
 }

@@ -102,3 +102,25 @@ def test_a_given_type_holds_for_every_operand_of_that_type(seam, r):
             wgrad(h, dw_type=code)
     with pytest.raises(TypeError):
         wgrad(h, f)
+
+
+@pytest.mark.parametrize("dtype, shape, code, ld", [
+    (torch.uint8, (4, 16), 2, 8), (torch.uint8, (4, 40), 2, 20), (torch.uint8, (4, 32), 0, 8), (torch.int16, (4, 8), 1, 8), (torch.int16, (4, 24), 2, 24),
+    (torch.int32, (4, 4), 2, 8), (torch.int32, (4, 12), 0, 12), (torch.int8, (4, 17), 2, None), (torch.uint8, (4, 34), 0, None), (torch.uint8, (4, 14), 2, None)])
+def test_the_pitch_of_storage_of_another_kind_is_in_elements_of_the_given_type(seam, r, dtype, shape, code, ld):
+    x = torch.zeros(shape, dtype=dtype)
+    calls = {"out": (lambda: seam.i8_restore(r, 0, -1, A, A, x, 8, 4, 0, 0, code, 0), 1),
+             "x": (lambda: seam.i8_quantize(r, 0, -1, x, A, A, 8, 4, False, 0, 0, code, 0), 0),
+             "y": (lambda: seam.i8_linear(r, 0, -1, A, A, A, A, x, 8, 4, 16, None, 0, 0, 0, code, 0), 2),
+             "sum": (lambda: seam.i8_rmsnorm(r, 0, -1, A, A, A, A, 8, 4, None, x, 1e-6, 0, 0, 0, 0, code, 0), 3),
+             "residual": (lambda: seam.i8_rmsnorm(r, 0, -1, A, A, A, A, 8, 4, x, None, 1e-6, 0, 0, 0, 0, code, 0), 1),
+             "dw": (lambda: seam.i8_wgrad(r, 0, -1, A, A, A, x, 8, 4, 16, None, 1.0, 0.0, 0, 0, 0, 0, 2, code, 0), 3),
+             "c": (lambda: seam.i8_wgrad(r, 0, -1, A, A, A, A, 8, 4, 16, x, 1.0, 1.0, 0, 0, 0, 0, 2, code, 0), 2)}
+    if code:
+        calls["dy"] = (lambda: seam.i8_wgrad(r, 0, -1, A, A, x, A, 16, 8, 4, None, 1.0, 0.0, 0, 0, 0, 0, code, 0, 0), 1)
+    for what, (call, at) in calls.items():
+        if ld is None:
+            with pytest.raises(ValueError, match="apart"):
+                call()
+        else:
+            assert call() == 0 and (ctypes.c_uint32 * 4).in_dll(seam.state, "seam_ld")[at] == ld, what
