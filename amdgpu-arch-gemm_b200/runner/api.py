@@ -140,7 +140,7 @@ def _native():
         spec = importlib.util.spec_from_file_location("_sgemm_native", NATIVE_PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
-        module.setup(_type_codes, _type_code)
+        module.setup(_type_code)
         _native_module = module
     return _native_module
 

@@ -29,7 +29,7 @@ def seam(tmp_path_factory):
     spec = importlib.util.spec_from_file_location("_sgemm_native", out)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    module.setup(api._type_codes, api._type_code)
+    module.setup(api._type_code)
     module.state = ctypes.CDLL(str(out))
     return module
 
@@ -124,3 +124,35 @@ def test_the_pitch_of_storage_of_another_kind_is_in_elements_of_the_given_type(s
                 call()
         else:
             assert call() == 0 and (ctypes.c_uint32 * 4).in_dll(seam.state, "seam_ld")[at] == ld, what
+
+
+class ByName:
+    """A tensor of a type without DLPack's table: it is asked by method and attribute names."""
+
+    def __init__(self, tensor):
+        self._t = tensor
+        for name in ("data_ptr", "get_device", "is_contiguous", "stride", "element_size"):
+            setattr(self, name, getattr(tensor, name))
+        self.dtype, self.shape = tensor.dtype, tensor.shape
+
+
+def test_tensors_are_read_alike_by_dlpack_and_by_name(seam, r):
+    """Shapes, strides, types and the refusals that follow from them, through both ways of asking; Parameters and views among them."""
+    def outcome(x, type_code=None, k=8):
+        try:
+            seam.i8_restore(r, 0, -1, A, A, x, k, 4, 0, 0, type_code, 0)
+            return (ctypes.c_uint32 * 4).in_dll(seam.state, "seam_ld")[1]
+        except (TypeError, ValueError) as e:
+            return type(e).__name__
+
+    base = torch.zeros(6, 40)
+    views = [base, base[:4, :8], base[::2, 3:11], base[:, :8].t(), base.view(3, 2, 40)[:, :, :8], base.view(2, 3, 40)[:, :2, :8], base[0], base[:1, :8],
+             base[:1].expand(4, 40), base.double(), base.half(), base.bfloat16()[:, ::2], base.int(), torch.nn.Parameter(base), torch.zeros(4, 1, 8),
+             torch.zeros(1, 4, 8).transpose(0, 1), torch.zeros(1, 1, 1, 40), base.to(torch.int8), torch.zeros(5, 1, 8, 1)[..., 0], base.requires_grad_()[1:]]
+    seen = set()
+    for x in views:
+        for code in (None, 0, 1, 2):
+            got = outcome(x, code)
+            assert got == outcome(ByName(x), code), (tuple(x.shape), x.stride(), x.dtype, code)
+            seen.add(got)
+    assert {"TypeError", "ValueError", 8, 40, 80} <= seen
