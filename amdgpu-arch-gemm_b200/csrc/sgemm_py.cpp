@@ -11,6 +11,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include "sgemm_i8_params.hpp"
 #include "sgemm_runner.h"
 
 namespace {
@@ -89,6 +90,15 @@ struct Operand {
             dense *= shape[d];
         }
         return true;
+    }
+    // elements from the first to the last one
+    uint64_t extent() const {
+        uint64_t n = 1;
+        for (int d = 0; d < ndim; ++d) {
+            if (shape[d] == 0) return 0;
+            n += (uint64_t)(shape[d] - 1) * (uint64_t)stride[d];
+        }
+        return n;
     }
     // Fills in what the object tells about itself; true when it did so by DLPack (`t` then holds its device and address too).
     bool read(PyObject *object, DlTensor &t) {
@@ -209,6 +219,18 @@ struct Call {
         ok = false;
         return dense;
     }
+    // A matrix of `rows` rows of `length` elements `ld` apart must end inside its tensor, a vector is one row; `code` as in ld().  (What a call
+    // does not touch has no rows; an `ld` below `length` is refused by the call itself.)
+    void extent(const Operand &o, uint32_t rows, uint32_t ld, uint32_t length, int code = -1) {
+        if (!ok || o.ndim < 0 || rows == 0 || length == 0 || ld < length) return;
+        const uint64_t need = (uint64_t)(rows - 1) * ld + length;
+        uint64_t have = o.extent();
+        if (code >= 0 && o.code != code && o.bytes > 0) have = have * (uint64_t)o.bytes / (code == 0 ? 4 : 2);
+        if (have >= need) return;
+        PyErr_Format(PyExc_ValueError, "%s holds %llu elements, the call reaches over %llu", o.name, (unsigned long long)have, (unsigned long long)need);
+        ok = false;
+    }
+    void extent(const Operand &vector, uint32_t length) { extent(vector, 1, length, length); }
     float f32(PyObject *x) {
         if (!ok) return 0.0f;
         const double v = PyFloat_AsDouble(x);
@@ -264,6 +286,14 @@ NATIVE_BEGIN(i8_linear, 14)
     const uint32_t m = c.u32(a[5]), tokens = c.u32(a[6]), k = c.u32(a[7]);
     const int type = c.type(y, a[12]), y_given = given(a[12], type);
     const uint32_t ldw = c.ld(a[9], w, k), ldx = c.ld(a[10], x, k), ldy = c.ld(a[11], y, m, y_given);
+    if (m && tokens && k <= I8_MAX_K) {
+        c.extent(w, m, ldw, k);
+        c.extent(ws, m);
+        c.extent(x, tokens, ldx, k);
+        c.extent(xs, tokens);
+        c.extent(y, tokens, ldy, m, y_given);
+        c.extent(bias, m);
+    }
     void *stream = c.ptr(a[13]);
 NATIVE_END(sgemm_i8_linear(h, as<int8_t>(w), as<float>(ws), as<int8_t>(x), as<float>(xs), as<float>(bias), y.p, type, m, tokens, k, ldw, ldx, ldy, stream))
 
@@ -276,6 +306,9 @@ NATIVE_BEGIN(i8_quantize, 10)
     const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]);
     const int pow2 = c.flag(a[5]), type = c.type(x, a[8]), x_given = given(a[8], type);
     const uint32_t ldx = c.ld(a[6], x, k, x_given), ldq = c.ld(a[7], q, k);
+    c.extent(x, rows, ldx, k, x_given);
+    c.extent(q, rows, ldq, k);
+    c.extent(s, rows);
     void *stream = c.ptr(a[9]);
 NATIVE_END(sgemm_i8_quantize(h, x.p, type, as<int8_t>(q), as<float>(s), k, rows, ldx, ldq, pow2, stream))
 
@@ -288,6 +321,9 @@ NATIVE_BEGIN(i8_restore, 9)
     const uint32_t k = c.u32(a[3]), rows = c.u32(a[4]);
     const int type = c.type(out, a[7]), out_given = given(a[7], type);
     const uint32_t ldq = c.ld(a[5], q, k), ldo = c.ld(a[6], out, k, out_given);
+    c.extent(q, rows, ldq, k);
+    c.extent(s, k ? rows : 0);
+    c.extent(out, rows, ldo, k, out_given);
     void *stream = c.ptr(a[8]);
 NATIVE_END(sgemm_i8_restore(h, as<int8_t>(q), as<float>(s), out.p, type, k, rows, ldq, ldo, stream))
 
@@ -304,6 +340,12 @@ NATIVE_BEGIN(i8_rmsnorm, 15)
     const uint32_t k = c.u32(a[4]), rows = c.u32(a[5]);
     const float eps = c.f32(a[8]);
     const uint32_t ldx = c.ld(a[9], x, k, x_given), ldr = c.ld(a[10], res, k, x_given), ldq = c.ld(a[11], q, k), lds = c.ld(a[12], sum, k, x_given);
+    c.extent(x, rows, ldx, k, x_given);
+    c.extent(g, rows ? 1 : 0, k, k, x_given);
+    c.extent(q, rows, ldq, k);
+    c.extent(s, rows);
+    c.extent(res, rows, ldr, k, x_given);
+    c.extent(sum, rows, lds, k, x_given);
     void *stream = c.ptr(a[14]);
 NATIVE_END(sgemm_i8_rmsnorm(h, x.p, res.p, g.p, type, eps, as<int8_t>(q), as<float>(s), sum.p, k, rows, ldx, ldr, ldq, lds, stream))
 
@@ -320,6 +362,13 @@ NATIVE_BEGIN(i8_wgrad, 17)
     const float alpha = c.f32(a[8]), beta = c.f32(a[9]);
     const uint32_t ldq = c.ld(a[10], q, m), lddy = c.ld(a[11], dy, channels, dy_given), ldc = c.ld(a[12], prior, m, dw_given),
                    lddw = c.ld(a[13], dw, m, dw_given);
+    if (m && channels) {
+        c.extent(q, tokens, ldq, m);
+        c.extent(s, tokens);
+        c.extent(dy, tokens, lddy, channels, dy_given);
+        c.extent(dw, channels, lddw, m, dw_given);
+        if (beta != 0.0f) c.extent(prior, channels, ldc, m, dw_given);
+    }
     void *stream = c.ptr(a[16]);
 NATIVE_END(sgemm_i8_wgrad(h, as<int8_t>(q), as<float>(s), dy.p, dy_type, prior.p, dw.p, dw_type, alpha, beta, m, channels, tokens, ldq, lddy, ldc, lddw, stream))
 

@@ -292,7 +292,8 @@ class SgemmRunner:
         return x.data_ptr()
 
     # Operands are tensors on the handle's GPU or addresses (their element type then goes with ..._type: 0 FP32, 1 FP16, 2 BF16).  A leading
-    # dimension of 0 is the distance of a tensor's rows (of all its dimensions but the last), and for addresses the length of a row.
+    # dimension of 0 is the distance of a tensor's rows (of all its dimensions but the last), and for addresses the length of a row.  A tensor
+    # that ends before the last element the call would touch is refused (ValueError).
     def _i8(self, name: str, *args):
         if not self._h:
             raise SgemmError(-1, "sgemm_" + name, "the handle is closed")

@@ -156,3 +156,88 @@ def test_tensors_are_read_alike_by_dlpack_and_by_name(seam, r):
             assert got == outcome(ByName(x), code), (tuple(x.shape), x.stride(), x.dtype, code)
             seen.add(got)
     assert {"TypeError", "ValueError", 8, 40, 80} <= seen
+
+
+def shapes(**kw):
+    """The operands of one call each as (shape, dtype), all exactly as large as the call needs; `kw` replaces some."""
+    i8, f32, bf16 = torch.int8, torch.float32, torch.bfloat16
+    t = {"w": ((16, 32), i8), "w_scale": ((16,), f32), "x": ((4, 32), i8), "x_scale": ((4,), f32), "y": ((4, 16), bf16), "bias": ((16,), f32),
+         "a": ((4, 32), bf16), "gamma": ((32,), bf16), "q": ((4, 32), i8), "scale": ((4,), f32), "residual": ((4, 32), bf16), "total": ((4, 32), bf16),
+         "dy": ((4, 16), bf16), "dw": ((16, 32), f32), "c": ((16, 32), f32)}
+    return {k: kw[k] if k in kw else torch.zeros(v[0], dtype=v[1]) for k, v in t.items()}
+
+
+RUN = {
+    "i8_linear": (("w", "w_scale", "x", "x_scale", "y", "bias"), lambda s, r, t, m=16, n=4, k=32: s.i8_linear(
+        r, 0, -1, t["w"], t["w_scale"], t["x"], t["x_scale"], t["y"], m, n, k, t["bias"], 0, 0, 0, None, 0)),
+    "i8_quantize": (("a", "q", "scale"), lambda s, r, t, k=32, n=4: s.i8_quantize(r, 0, -1, t["a"], t["q"], t["scale"], k, n, False, 0, 0, None, 0)),
+    "i8_restore": (("q", "scale", "a"), lambda s, r, t, k=32, n=4: s.i8_restore(r, 0, -1, t["q"], t["scale"], t["a"], k, n, 0, 0, None, 0)),
+    "i8_rmsnorm": (("a", "gamma", "q", "scale", "residual", "total"), lambda s, r, t, k=32, n=4: s.i8_rmsnorm(
+        r, 0, -1, t["a"], t["gamma"], t["q"], t["scale"], k, n, t["residual"], t["total"], 1e-6, 0, 0, 0, 0, None, 0)),
+    "i8_wgrad": (("q", "scale", "dy", "dw", "c"), lambda s, r, t, m=32, n=16, tokens=4, beta=1.0: s.i8_wgrad(
+        r, 0, -1, t["q"], t["scale"], t["dy"], t["dw"], m, n, tokens, t["c"], 1.0, beta, 0, 0, 0, 0, None, None, 0)),
+}
+
+
+@pytest.mark.parametrize("form", [lambda x: x, ByName], ids=["dlpack", "by_name"])
+@pytest.mark.parametrize("name, operand", [(n, o) for n, (operands, _) in RUN.items() for o in operands])
+def test_a_tensor_that_ends_before_the_call_does_is_refused(seam, r, name, operand, form):
+    """One element less, or one row less, than the call reads or writes; more than that, and the same rows inside a wider tensor, are served."""
+    run = RUN[name][1]
+    full = shapes()[operand]
+    assert run(seam, r, shapes()) == 0
+    short = [full.reshape(-1)[:-1]] if full.dim() == 1 else [full[:-1], full.reshape(-1)[:-1], torch.zeros(4 * full.shape[0], 2 * full.shape[1], dtype=full.dtype)[:full.shape[0] - 1, :full.shape[1]],
+                                                              torch.zeros(full.shape[0], full.shape[1] + 8, dtype=full.dtype)[:, :full.shape[1] - 1]]
+    calls = value(seam, "seam_calls")
+    for x in short:
+        with pytest.raises(ValueError, match=r"elements, the call reaches over \d+"):
+            run(seam, r, shapes(**{operand: form(x)}))
+    assert value(seam, "seam_calls") == calls
+    if full.dim() == 1:
+        enough = [torch.zeros(full.shape[0] + 3, dtype=full.dtype), full[None], full[:, None]]
+    else:
+        enough = [torch.zeros(full.shape[0] + 1, full.shape[1], dtype=full.dtype), full.reshape(-1), full[None], full[:, None], full.reshape(2, -1, full.shape[1]),
+                  torch.zeros(full.shape[0], full.shape[1] + 8, dtype=full.dtype)[:, :full.shape[1]], torch.zeros(full.shape[0], full.shape[1] + 8, dtype=full.dtype)]
+    for x in enough:
+        assert run(seam, r, shapes(**{operand: form(x)})) == 0
+    if operand not in ("y", "a", "dy", "dw"):        # (an address comes with its type)
+        assert run(seam, r, shapes(**{operand: A})) == 0
+
+
+def test_extents_of_given_leading_dimensions_and_of_storage_of_another_kind(seam, r):
+    flat = torch.zeros(3 * 40 + 32, dtype=torch.int8)
+
+    def restore(q, ldq, out=A, ldo=0, code=0):
+        return seam.i8_restore(r, 0, -1, q, A, out, 32, 4, ldq, ldo, code, 0)
+
+    assert restore(flat, 40) == 0 and restore(flat.reshape(8, 19), 40) == 0
+    for q, ldq in ((flat, 41), (flat[1:], 40), (flat[:32].expand(4, 32), 32), (flat[:32].expand(4, 32), 40)):
+        with pytest.raises(ValueError, match="reaches over"):
+            restore(q, ldq)
+    raw = torch.zeros(4 * 64, dtype=torch.uint8)                  # 32 BF16 elements of 4 rows, or 16 FP32 ones
+    assert restore(A, 0, raw, 0, 2) == 0 and restore(A, 0, raw.view(4, 64), 0, 2) == 0
+    with pytest.raises(ValueError, match="reaches over"):
+        restore(A, 0, raw, 0, 0)
+    with pytest.raises(ValueError, match="reaches over"):
+        restore(A, 0, raw[:-1], 0, 2)
+
+
+def test_what_a_call_does_not_read_may_be_missing_or_empty(seam, r):
+    """No tokens, no channels, no features; C beside beta 0; and what the C call refuses by itself reaches it."""
+    none = {k: v.reshape(-1)[:0] for k, v in shapes().items()}
+    linear, quantize, restore, rms, wgrad = (RUN[n][1] for n in ("i8_linear", "i8_quantize", "i8_restore", "i8_rmsnorm", "i8_wgrad"))
+    assert linear(seam, r, none, n=0) == 0 and linear(seam, r, none, m=0) == 0
+    assert quantize(seam, r, none, n=0) == 0 and restore(seam, r, none, n=0) == 0 and restore(seam, r, none, k=0) == 0 and rms(seam, r, none, n=0) == 0
+    assert wgrad(seam, r, none, n=0) == 0 and wgrad(seam, r, none, m=0) == 0
+    t = shapes(q=none["q"], scale=none["scale"], dy=none["dy"])
+    assert wgrad(seam, r, t, tokens=0) == 0
+    assert wgrad(seam, r, shapes(c=none["c"]), beta=0.0) == 0
+    assert quantize(seam, r, shapes(q=none["q"], a=none["a"]), k=0) == 0
+    with pytest.raises(ValueError, match="scale holds 0"):
+        quantize(seam, r, none, k=0)                       # scales of empty rows are written
+    with pytest.raises(ValueError, match="w_scale holds 0"):
+        linear(seam, r, shapes(w_scale=none["w_scale"]), k=0)
+    assert linear(seam, r, shapes(w=none["w"], x=none["x"]), k=0) == 0
+    t = shapes()
+    assert seam.i8_linear(r, 0, -1, t["w"], t["w_scale"], t["x"], t["x_scale"], t["y"], 16, 4, 131072, None, 131072, 131072, 0, None, 0) == 0
+    assert seam.i8_linear(r, 0, -1, t["w"], t["w_scale"], t["x"], t["x_scale"], t["y"], 16, 4, 32, None, 31, 0, 0, None, 0) == 0
