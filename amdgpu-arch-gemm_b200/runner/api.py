@@ -14,6 +14,7 @@ import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 from typing import Optional, Tuple
 
@@ -103,8 +104,10 @@ _lib: Optional[ctypes.CDLL] = None
 
 
 def build_library(force: bool = False) -> Path:
-    """Run the Makefile beside this file (g++ and nvcc; needs the CUDA toolkit headers, not a GPU)."""
-    if force or not LIB_PATH.exists() or not RUNNER_PATH.exists() or not NATIVE_PATH.exists():
+    """Run the Makefile beside this file (g++ and nvcc; needs the CUDA toolkit headers, not a GPU).  The binding of the ``i8_*``
+    methods is built too where Python's headers are."""
+    headers = (Path(sysconfig.get_paths()["include"]) / "Python.h").exists()
+    if force or not LIB_PATH.exists() or not RUNNER_PATH.exists() or (headers and not NATIVE_PATH.exists()):
         env = dict(os.environ, PYTHON=sys.executable)
         env.pop("CXX", None)
         subprocess.run(["make", "-C", str(Path(__file__).resolve().parent), "-s"] + (["-B"] if force else []),
@@ -136,7 +139,8 @@ def _native():
     if _native_module is None:
         lib()
         if not NATIVE_PATH.exists():
-            raise SgemmError(-5, "_sgemm_native", f"{NATIVE_PATH} is not built; run __graft_entry__.build() or make -C {PKG_DIR / 'runner'}")
+            raise SgemmError(-5, "_sgemm_native", f"{NATIVE_PATH} is not built; run __graft_entry__.build() or make -C {PKG_DIR / 'runner'} "
+                                                 f"(needs Python's headers)")
         spec = importlib.util.spec_from_file_location("_sgemm_native", NATIVE_PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
