@@ -21,7 +21,7 @@ from typing import Optional, Tuple
 PKG_DIR = Path(__file__).resolve().parent.parent
 LIB_PATH = PKG_DIR / "build" / "libsgemm_runner.so"
 RUNNER_PATH = PKG_DIR / "build" / "GeneratorRunner"
-NATIVE_PATH = PKG_DIR / "build" / "_sgemm_native.so"
+NATIVE_PATH = PKG_DIR / "build" / ("_sgemm_native" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 _f32p = ctypes.POINTER(ctypes.c_float)
 _u32 = ctypes.c_uint32

@@ -41,3 +41,10 @@ def test_a_missing_binding_is_built_only_where_it_can_be(monkeypatch, tmp_path):
     (tmp_path / "Python.h").write_text("")
     api.build_library()
     assert len(calls) == 1
+
+
+def test_the_bindings_name_carries_the_interpreters_tag(monkeypatch):
+    """A module built for one Python must not be loaded by another: its file is named as import names extension modules."""
+    suffix = api.sysconfig.get_config_var("EXT_SUFFIX")
+    assert suffix != ".so" and api.NATIVE_PATH.name == "_sgemm_native" + suffix
+    assert f"-o ../build/_sgemm_native{suffix} " in commands()
