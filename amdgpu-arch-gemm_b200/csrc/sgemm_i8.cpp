@@ -103,28 +103,37 @@ struct LinearPlan {
     uint32_t parts = 1;
 };
 
-// Estimated nanoseconds of a call on each kernel, fitted to calls back to back on a B200 (captured graphs, weights out of L2); the
-// estimates meet the measured times of 17 shapes between (1, 4096, 4096) and (2048, 4096, 4096) within 15 %.  What matters is where
-// they cross: (tokens, channels, features) = (509, 4096, 4096) takes 14.9 us on 256 x 256 tiles, 10.8 on 256 x 128
-// and 14.2 on 128 x 128; (1024, 4096, 4096) 15.8, 17.2 and 26.8; (64, 4096, 4096) 14.8, 10.0 and, cut in 4 parts, 9.2.
+// Estimated nanoseconds of a call on each kernel, fitted to calls back to back on a B200 (captured graphs, weights out of L2).  What matters
+// is where they cross: (tokens, channels, features) = (509, 4096, 4096) takes 14.9 us on 256 x 256 tiles, 10.8 on 256 x 128
+// and 14.2 on 128 x 128; (1024, 4096, 4096) 15.8, 17.2 and 26.8; (64, 4096, 4096) 14.8, 10.0 and, cut in 4 parts, 9.2.  Over 112 shapes of 4096 to
+// 151936 channels, 2048 to 28672 features and 1 to 128 tokens the kernel of the least estimate is within 10 % of the fastest of all, 0.4 % on
+// average.  (Over 320 random ones, whose features end inside a 128-byte line, its time is up to 23 % above that of the pairs: the
+// estimates know nothing of the lines.)
 //   pairs: set-up and the first loads, then so many waves of tiles with a stage every 320 ns (256 x 256) or 190 (256 x 128)
 uint64_t pair_ns(uint64_t tiles, uint32_t pairs, uint32_t stages, bool half) {
     const uint64_t waves = (tiles + pairs - 1) / pairs;
     return half ? 4400 + waves * stages * 190 : 5000 + waves * stages * 320;
 }
+//   ... and never below the trip of its `bytes` from memory, which with the few large tiles of wide outputs is a little slower than with the
+//   few-token kernels' many: 256 x 128 tiles against 128 x 16 take 47.6 us and 41.5 for (1, 28672, 8192), 15.1 and 11.7 for (1, 12288, 4096);
+//   against 128 x 64 tiles 45.7 and 44.6 for (64, 28672, 8192), 13.1 and 13.9 for (64, 12288, 4096)
+uint64_t pair_trip_ns(uint64_t bytes) { return 4500 + bytes / 6000; }
 //   few tokens: a stage's cost is the latency of its loads over the depth of the ring; a cut adds the cluster's barriers and the sum over
-//   the parts, and is limited by how many clusters the device holds (148 SMs in uneven groups); never below the weights' trip from memory
+//   the parts, and is limited by how many clusters the device holds (148 SMs in uneven groups): a second wave of clusters begins when the first
+//   has added up, (1, 28672, 4096) takes 22.2 us whole, 25.8 in 2 parts, 40.3 in 8.  Never below the trip from memory; where that decides, the
+//   cut with more loads under way is a little faster
 uint64_t few_ns(const FewKernel &f, uint64_t tiles, uint32_t stages, uint32_t parts, uint32_t sms, uint64_t bytes) {
     const uint32_t per_sm = f.tile_n <= 64 ? 2 : 1;
-    const uint64_t slots = per_sm * (parts == 1 ? sms : parts == 2 ? sms / 2 : parts == 4 ? sms * 33 / 148 : sms * 15 / 148);
-    const uint64_t waves = (tiles + std::max<uint64_t>(slots, 1) - 1) / std::max<uint64_t>(slots, 1);
+    const uint64_t slots = std::max<uint64_t>(per_sm * (parts == 1 ? sms : parts == 2 ? sms / 2 : parts == 4 ? sms * 33 / 148 : sms * 15 / 148), 1);
+    const uint64_t waves = (tiles + slots - 1) / slots;
     const uint64_t stage = f.tile_n == 128 ? 345 : f.tile_n == 64 ? 317 : f.tile_n == 32 ? 270 : 236;
     const uint64_t ns = 2000 + waves * ceil_div(stages, parts) * stage + (parts > 1 ? 1100 + 40ull * f.tile_n : 0);
-    return std::max<uint64_t>(ns, 3500 + bytes / 6000) + ns / 8;   // (where memory decides, the cut with more loads under way)
+    const uint64_t trip = 3500 + bytes / 6600 + (parts > 1 ? 30 : 10) * f.tile_n;
+    return std::max(ns, trip) + ns / 8 + (waves - 1) * (parts == 1 ? 20 * f.tile_n : trip > ns ? 2000 : 0);
 }
 
 int plan_linear(sgemm_handle *h, const I8View &v, const void *w, const void *x, uint32_t m, uint32_t n, uint32_t k,
-                uint32_t ldw, uint32_t ldx, LinearPlan *p) {
+                uint32_t ldw, uint32_t ldx, int y_type, LinearPlan *p) {
     const bool tma = aligned(w, 16) && aligned(x, 16) && ldw % 16 == 0 && ldx % 16 == 0;
     if (v.force_variant != 0 && v.force_variant != 2 && (!tma || k == 0))
         return refuse(h, SGEMM_ERR_UNSUPPORTED, "sgemm_i8_linear",
@@ -138,7 +147,8 @@ int plan_linear(sgemm_handle *h, const I8View &v, const void *w, const void *x, 
     const uint32_t sms = (uint32_t)std::max(v.sm_count, 2), pairs = sms / kSmsPerPair, stages = ceil_div(k, I8_BK);
     const uint64_t full = pair_ns((uint64_t)ceil_div(m, 256) * ceil_div(n, v.tile_n), pairs, stages, false);
     const uint64_t half = pair_ns((uint64_t)ceil_div(m, 256) * ceil_div(n, I8_HALF_BN), pairs, stages, true);
-    uint64_t best = std::min(full, half);
+    const uint64_t bytes = (uint64_t)m * k + (uint64_t)n * k + (uint64_t)m * n * type_bytes(y_type);
+    uint64_t best = std::max(std::min(full, half), pair_trip_ns(bytes));
     if (half < full) p->index = kHalf;
     // the few-token kernel whose tile holds all tokens (the widest takes more than one tile only when it is forced)
     const FewKernel *few = &kFew[3];
@@ -150,7 +160,7 @@ int plan_linear(sgemm_handle *h, const I8View &v, const void *w, const void *x, 
     for (uint32_t parts = 1; parts <= 8; parts *= 2) {
         if (v.split_k > 0 && parts != (v.split_k >= 8 ? 8u : v.split_k >= 4 ? 4u : v.split_k >= 2 ? 2u : 1u)) continue;
         if (v.split_k == 0 && parts > 1 && stages < 2 * parts) break;
-        const uint64_t ns = few_ns(*few, tiles, stages, parts, sms, (uint64_t)m * k);
+        const uint64_t ns = few_ns(*few, tiles, stages, parts, sms, bytes);
         if (ns < best) {
             best = ns;
             p->index = few->index;
@@ -253,7 +263,7 @@ SGEMM_API int sgemm_i8_linear(sgemm_handle *h, const int8_t *dW, const float *dW
         return refuse(h, SGEMM_ERR_INVALID_ARGUMENT, op, "scales and bias are FP32 and must be aligned to 4 bytes");
     I8Scope scope(h);
     LinearPlan p;
-    if ((rc = plan_linear(h, v, dW, dX, m, n, k, ldw, ldx, &p))) return rc;
+    if ((rc = plan_linear(h, v, dW, dX, m, n, k, ldw, ldx, y_type, &p))) return rc;
     LinearArgs a{dW, dWscale, dX, dXscale, dBias, dY, v.status, m, n, k, ldw, ldx, ldy, (uint32_t)y_type, 0, 0};
     const bool pair = p.index == kLinear || p.index == kHalf;
     const uint32_t tile_m = pair ? 256 : p.few ? I8_BM : I8_SIMT_TILE;
