@@ -282,7 +282,8 @@ int sgemm_narrow16(sgemm_handle *h, const float *dsrc, void *ddst, uint64_t coun
 
 /* Linear layer: Y[i, j] = fp32(sum_k W[k, i] * X[k, j]) * x_scale[j] * w_scale[i] (+ bias[i]) for M channels and N tokens, W
  * K x M, X K x N, Y M x N (ldy >= M) in y_type, rounded once.  bias: M FP32 values or NULL.  The integer sum is exact
- * (K <= 131071, larger is SGEMM_ERR_INVALID_ARGUMENT), so results do not depend on tiles or cuts. */
+ * (K <= 131071, larger is SGEMM_ERR_INVALID_ARGUMENT), so results do not depend on tiles or cuts.  The products are FP32 from left to
+ * right: where the sum times x_scale alone leaves FP32 (possible for x_scale above 2^97), so does Y. */
 int sgemm_i8_linear(sgemm_handle *h, const int8_t *dW, const float *dWscale, const int8_t *dX, const float *dXscale,
                     const float *dBias, void *dY, int y_type, uint32_t m, uint32_t n, uint32_t k,
                     uint32_t ldw, uint32_t ldx, uint32_t ldy, void *stream);
@@ -301,7 +302,8 @@ int sgemm_i8_restore(sgemm_handle *h, const int8_t *dQ, const float *dScale, voi
 
 /* Root-mean-square norm with the residual's addition and an 8-bit result, per column of X (K x N in x_type, K > 0):
  * h = x + residual and p = h * gamma in FP32; scale = P / 127 * rsqrt(mean h^2 + eps) with P = max |p|; q = round(127 p / P).
- * dResidual may be NULL (h = x).  dSum, unless NULL, receives h rounded to x_type and may be dResidual or dX itself (same
+ * eps is a finite number >= 0.  The mean is that of the definition however large or small h is, as far as the scale itself is an FP32
+ * number.  dResidual may be NULL (h = x).  dSum, unless NULL, receives h rounded to x_type and may be dResidual or dX itself (same
  * leading dimension).  gamma, residual and sum have x_type.  Columns as in sgemm_i8_quantize when P is 0 or out of range. */
 int sgemm_i8_rmsnorm(sgemm_handle *h, const void *dX, const void *dResidual, const void *dGamma, int x_type, float eps,
                      int8_t *dQ, float *dScale, void *dSum, uint32_t k, uint32_t n, uint32_t ldx, uint32_t ldr,
