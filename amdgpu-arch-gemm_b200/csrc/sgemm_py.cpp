@@ -108,7 +108,7 @@ struct Operand {
                 ndim = t.ndim;
                 shape = t.shape;
                 stride = t.strides;
-                bytes = t.bits / 8;
+                bytes = (t.bits * t.lanes + 7) / 8;
                 if (t.lanes == 1) code = t.code == 2 && t.bits == 32 ? 0 : t.code == 2 && t.bits == 16 ? 1 : t.code == 4 && t.bits == 16 ? 2 : t.code == 0 && t.bits == 8 ? 3 : -1;
                 return true;
             }
@@ -154,7 +154,8 @@ struct Call {
             return o;
         }
         DlTensor t;
-        if (o.read(x, t) && (device < 0 ? t.device_type == 1 : t.device_type == 2 && t.device_id == device) && (code < 0 || o.code == code) && o.contiguous()) {
+        if (o.read(x, t) && (device < 0 ? t.device_type == 1 : t.device_type == 2 && t.device_id == device) && (code < 0 || o.code == code) && o.contiguous() &&
+            t.data) {   // (a type may give no address, as wrappers without storage do: they say what is wrong when asked by name)
             o.p = static_cast<char *>(t.data) + t.byte_offset;
             return o;
         }
@@ -226,7 +227,13 @@ struct Call {
         const uint64_t need = (uint64_t)(rows - 1) * ld + length;
         uint64_t have = o.extent();
         if (code >= 0 && o.code != code && o.bytes > 0) have = have * (uint64_t)o.bytes / (code == 0 ? 4 : 2);
-        if (have >= need) return;
+        if (have >= need) {
+            if (!o.p) {   // NULL would be an operand that was left out
+                PyErr_Format(PyExc_ValueError, "%s has no storage", o.name);
+                ok = false;
+            }
+            return;
+        }
         PyErr_Format(PyExc_ValueError, "%s holds %llu elements, the call reaches over %llu", o.name, (unsigned long long)have, (unsigned long long)need);
         ok = false;
     }

@@ -43,8 +43,10 @@ def test_a_missing_binding_is_built_only_where_it_can_be(monkeypatch, tmp_path):
     assert len(calls) == 1
 
 
-def test_the_bindings_name_carries_the_interpreters_tag(monkeypatch):
+def test_the_bindings_name_carries_the_interpreters_tag():
     """A module built for one Python must not be loaded by another: its file is named as import names extension modules."""
     suffix = api.sysconfig.get_config_var("EXT_SUFFIX")
+    if not (Path(api.sysconfig.get_paths()["include"]) / "Python.h").exists():
+        pytest.skip("Python's headers are not here")
     assert suffix != ".so" and api.NATIVE_PATH.name == "_sgemm_native" + suffix
     assert f"-o ../build/_sgemm_native{suffix} " in commands()

@@ -241,3 +241,23 @@ def test_what_a_call_does_not_read_may_be_missing_or_empty(seam, r):
     t = shapes()
     assert seam.i8_linear(r, 0, -1, t["w"], t["w_scale"], t["x"], t["x_scale"], t["y"], 16, 4, 131072, None, 131072, 131072, 0, None, 0) == 0
     assert seam.i8_linear(r, 0, -1, t["w"], t["w_scale"], t["x"], t["x_scale"], t["y"], 16, 4, 32, None, 31, 0, 0, None, 0) == 0
+
+
+class Shell(torch.Tensor):
+    """A tensor without storage of its own, as wrapper subclasses are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, strides=inner.stride(), device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+@pytest.mark.parametrize("name, operand", [("i8_linear", "bias"), ("i8_rmsnorm", "residual"), ("i8_rmsnorm", "total"), ("i8_linear", "w"), ("i8_wgrad", "c")])
+def test_a_tensor_without_storage_is_not_taken_for_an_absent_one(seam, r, name, operand):
+    calls = value(seam, "seam_calls")
+    with pytest.raises((RuntimeError, TypeError, ValueError, NotImplementedError)):
+        RUN[name][1](seam, r, shapes(**{operand: Shell(shapes()[operand])}))
+    assert value(seam, "seam_calls") == calls
