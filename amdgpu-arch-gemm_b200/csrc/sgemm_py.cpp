@@ -121,13 +121,13 @@ struct Operand {
                 own[d] = PyLong_AsLongLong(PyTuple_GET_ITEM(sizes, d));
                 own[kMost + d] = PyLong_AsLongLong(PyTuple_GET_ITEM(strides, d));
             }
-            PyObject *size = PyErr_Occurred() ? nullptr : PyObject_CallMethodNoArgs(x, s_element_size);
-            if (size) bytes = PyLong_AsLongLong(size);
-            Py_XDECREF(size);
             if (!PyErr_Occurred()) {
                 ndim = n;
                 shape = own;
                 stride = own + kMost;
+                PyObject *size = PyObject_CallMethodNoArgs(x, s_element_size);   // (one without it has the call's elements)
+                if (size) bytes = PyLong_AsLongLong(size);
+                Py_XDECREF(size);
             }
         }
         Py_XDECREF(sizes);

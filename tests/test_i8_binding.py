@@ -261,3 +261,12 @@ def test_a_tensor_without_storage_is_not_taken_for_an_absent_one(seam, r, name, 
     with pytest.raises((RuntimeError, TypeError, ValueError, NotImplementedError)):
         RUN[name][1](seam, r, shapes(**{operand: Shell(shapes()[operand])}))
     assert value(seam, "seam_calls") == calls
+
+
+def test_an_object_that_tells_its_strides_only_by_name_keeps_its_pitch(seam, r):
+    x = ByName(torch.zeros(4, 40)[:, :8])
+    del x.element_size
+    assert seam.i8_restore(r, 0, -1, A, A, x, 8, 4, 0, 0, None, 0) == 0
+    assert (ctypes.c_uint32 * 4).in_dll(seam.state, "seam_ld")[1] == 40
+    with pytest.raises(ValueError, match="reaches over"):
+        seam.i8_restore(r, 0, -1, A, A, x, 8, 5, 0, 0, None, 0)
